@@ -5,6 +5,9 @@ Modules:
   dora_fused  fused compose / norm-assembly / autograd Function -- drop-in for
               peft.tuners.lora.dora_fused
   layer       DoraLinear, a stand-alone adapted linear wired like PEFT's
+  norms       layer norm and RMS norm, forward and backward
+  logprobs    log probabilities of given tokens, entropy, top alternatives, and the gradient
+  optim       AdamW over many tensors at once, moments in 32 or 8 bits
   _native     ctypes binding of libdora_b200.so (C ABI: include/dora_b200.h)
 """
 
@@ -21,3 +24,6 @@ from .dora_fused import (  # noqa: F401
     is_triton_available,
 )
 from .layer import DoraLinear  # noqa: F401
+from .logprobs import token_logprobs  # noqa: F401
+from .norms import LayerNorm, RMSNorm, layer_norm, rms_norm  # noqa: F401
+from .optim import AdamW  # noqa: F401

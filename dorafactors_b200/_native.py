@@ -60,6 +60,18 @@ SIGNATURES = {
     "dora_weight_norm_workspace_size": (_sz, [_i64, _i64, _i64, _int, _int, _int]),
     "dora_weight_norm": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _dbl, _vp, _vp, _vp, _sz, _vp]),
     "dora_weight_norm_dense": (_int, [_vp, _vp, _i64, _i64, _int, _int, _dbl, _vp, _vp]),
+    "dora_layer_norm_fwd": (_int, [_vp, _i64, _vp, _vp, _int, _dbl, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
+    "dora_rms_norm_fwd": (_int, [_vp, _i64, _vp, _int, _dbl, _vp, _vp, _i64, _i64, _int, _vp]),
+    "dora_layer_norm_bwd_workspace_size": (_sz, [_i64, _i64]),
+    "dora_layer_norm_bwd": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64,
+                                   _int, _vp]),
+    "dora_rms_norm_bwd": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _int, _vp]),
+    "dora_token_logprobs_fwd": (_int, [_vp, _i64, _vp, _i64, _dbl, _vp, _vp, _vp, _int, _vp, _vp, _i64, _i64, _int,
+                                       _vp]),
+    "dora_token_logprobs_bwd": (_int, [_vp, _i64, _vp, _i64, _dbl, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                       _int, _vp]),
+    "dora_adamw_step": (_int, [_vp, _i64, _int, _int, _dbl, _dbl, _dbl, _dbl, _dbl, _i64, _vp]),
+    "dora_adamw_decode": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
 _lib = None
@@ -401,3 +413,133 @@ def weight_norm_dense(W, L, scale: float, norm_out) -> None:
         ptr(W), ptr(L), out_f, in_f, dtype_code(W), dtype_code(L), float(scale), ptr(norm_out), stream_ptr(W.device)
     )
     check(code, "dora_weight_norm_dense")
+
+
+# ---------------------------------------------------------------------------
+# Norms, token log probabilities and AdamW.  Their smallest calls are short against
+# the host's own work, so addresses and streams go as plain integers.
+# ---------------------------------------------------------------------------
+def on_device(device: torch.device):
+    """Guard that makes ``device`` current where it is not (a launch goes to the current device)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+class _SameDevice:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def addr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def rows_of(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """``x`` as rows of its last dimension: (tensor that holds the data, rows, cols, row
+    stride).  Rows of a wider buffer are taken as they are; other layouts are copied."""
+    cols = x.shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // cols if cols else x.shape[:-1].numel(), cols, cols
+    if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+        return x, x.shape[0], cols, x.stride(0)
+    if x.ndim > 2 and x.stride(-1) == 1 and x.numel():
+        try:
+            v = x.view(-1, cols)
+        except RuntimeError:
+            v = None
+        if v is not None and v.stride(0) >= cols:
+            return v, v.shape[0], cols, v.stride(0)
+    x = x.contiguous()
+    return x, x.numel() // cols if cols else x.shape[:-1].numel(), cols, cols
+
+
+def layer_norm_fwd(x, rows, cols, ldx, weight, bias, w_code: int, eps: float, y, mean, rstd, rms: bool) -> None:
+    dev = x.device
+    lib = load_library()
+    with on_device(dev):
+        if rms:
+            code = lib.dora_rms_norm_fwd(x.data_ptr(), ldx, addr(weight), w_code, eps, y.data_ptr(), addr(rstd), rows,
+                                         cols, DTYPE_CODE[x.dtype], _raw_stream(dev))
+        else:
+            code = lib.dora_layer_norm_fwd(x.data_ptr(), ldx, addr(weight), addr(bias), w_code, eps, y.data_ptr(),
+                                           addr(mean), addr(rstd), rows, cols, DTYPE_CODE[x.dtype], _raw_stream(dev))
+    if code:
+        check(code, "dora_rms_norm_fwd" if rms else "dora_layer_norm_fwd")
+
+
+def layer_norm_bwd(dy, lddy, x, ldx, rows, cols, weight, w_code: int, mean, rstd, dx, dw, db, rms: bool) -> None:
+    dev = x.device
+    lib = load_library()
+    with on_device(dev):
+        ws, nbytes = None, 0
+        if dw is not None or db is not None:
+            nbytes = lib.dora_layer_norm_bwd_workspace_size(rows, cols)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        if rms:
+            code = lib.dora_rms_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, addr(weight), w_code, addr(rstd),
+                                         addr(dx), addr(dw), addr(ws), nbytes, rows, cols, DTYPE_CODE[x.dtype],
+                                         _raw_stream(dev))
+        else:
+            code = lib.dora_layer_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, addr(weight), w_code, addr(mean),
+                                           addr(rstd), addr(dx), addr(dw), addr(db), addr(ws), nbytes, rows, cols,
+                                           DTYPE_CODE[x.dtype], _raw_stream(dev))
+    if code:
+        check(code, "dora_rms_norm_bwd" if rms else "dora_layer_norm_bwd")
+
+
+def token_logprobs_fwd(logits, ld, targets, ignore_index: int, temperature: float, logprobs, lse, entropy, top_k: int,
+                       top_logprobs, top_indices, rows: int, vocab: int) -> None:
+    dev = logits.device
+    with on_device(dev):
+        code = load_library().dora_token_logprobs_fwd(
+            logits.data_ptr(), ld, targets.data_ptr(), ignore_index, temperature, logprobs.data_ptr(), lse.data_ptr(),
+            addr(entropy), top_k, addr(top_logprobs), addr(top_indices), rows, vocab, DTYPE_CODE[logits.dtype],
+            _raw_stream(dev))
+    if code:
+        check(code, "dora_token_logprobs_fwd")
+
+
+def token_logprobs_bwd(logits, ld, targets, ignore_index: int, temperature: float, lse, entropy, g_logprobs,
+                       g_entropy, g_lse, d_logits, ld_d: int, rows: int, vocab: int) -> None:
+    dev = logits.device
+    with on_device(dev):
+        code = load_library().dora_token_logprobs_bwd(
+            logits.data_ptr(), ld, targets.data_ptr(), ignore_index, temperature, lse.data_ptr(), addr(entropy),
+            addr(g_logprobs), addr(g_entropy), addr(g_lse), d_logits.data_ptr(), ld_d, rows, vocab,
+            DTYPE_CODE[logits.dtype], _raw_stream(dev))
+    if code:
+        check(code, "dora_token_logprobs_bwd")
+
+
+#: ``dora_adamw_tensor_t`` as a numpy record.
+ADAMW_TENSOR = [("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg_sq", "u8"), ("exp_avg_scale", "u8"),
+                ("exp_avg_sq_scale", "u8"), ("master", "u8"), ("numel", "i8"), ("key", "u4"), ("reserved", "u4")]
+
+
+def adamw_step(table, dtype: torch.dtype, state_bits: int, lr: float, betas, eps: float, weight_decay: float,
+               step: int, device: torch.device) -> None:
+    """``table``: a contiguous numpy array of ``ADAMW_TENSOR`` records."""
+    with on_device(device):
+        code = load_library().dora_adamw_step(table.ctypes.data, len(table), DTYPE_CODE[dtype], state_bits, lr,
+                                              betas[0], betas[1], eps, weight_decay, step, _raw_stream(device))
+    if code:
+        check(code, "dora_adamw_step")
+
+
+def adamw_decode(m_codes, m_scale, v_codes, v_scale, m, v) -> None:
+    dev = m.device
+    with on_device(dev):
+        code = load_library().dora_adamw_decode(m_codes.data_ptr(), m_scale.data_ptr(), v_codes.data_ptr(),
+                                                v_scale.data_ptr(), m.data_ptr(), v.data_ptr(), m.numel(),
+                                                _raw_stream(dev))
+    if code:
+        check(code, "dora_adamw_decode")

@@ -343,6 +343,109 @@ int dora_weight_norm(const void* W, const void* A, const void* B, int64_t out_fe
 int dora_weight_norm_dense(const void* W, const void* L, int64_t out_features, int64_t in_features, int w_dtype,
                            int l_dtype, double scale, void* norm_out, void* stream);
 
+/*
+ * Layer norm over the last dimension of x [rows x cols] (row stride ldx, unit column
+ * stride):  mean = sum x / cols, rstd = (sum (x - mean)^2 / cols + eps)^-1/2,
+ * y = (x - mean) * rstd * weight + bias.  y is contiguous in act_dtype; weight and bias
+ * (either may be NULL) are in w_dtype, which is act_dtype or DORA_DTYPE_F32; mean and
+ * rstd are fp32 [rows], NULL where they are not wanted.  y must not alias x.
+ */
+int dora_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, int w_dtype, double eps,
+                        void* y, void* mean, void* rstd, int64_t rows, int64_t cols, int act_dtype, void* stream);
+
+/* RMS norm: rstd = (sum x^2 / cols + eps)^-1/2, y = x * rstd * weight; else as above. */
+int dora_rms_norm_fwd(const void* x, int64_t ldx, const void* weight, int w_dtype, double eps, void* y, void* rstd,
+                      int64_t rows, int64_t cols, int act_dtype, void* stream);
+
+/* Bytes of workspace that either norm's backward needs for its column sums on the current device. */
+size_t dora_layer_norm_bwd_workspace_size(int64_t rows, int64_t cols);
+
+/*
+ * Backward of the norms.  With xh = (x - mean) * rstd and a = dy * weight:
+ *   dx = rstd * (a - mean(a) - xh * mean(a * xh))     (RMS norm: without mean(a))
+ *   d_weight = sum over rows of dy * xh, d_bias = sum over rows of dy   (in w_dtype)
+ * mean and rstd are what the forward gave.  Outputs that are NULL are not computed; dx is
+ * contiguous and must not alias an input.  The workspace (16-byte aligned, contents
+ * don't matter) is needed for d_weight and d_bias only.  Column sums are fp32 in a
+ * fixed order: results do not change from call to call.  With rows == 0 d_weight and
+ * d_bias are zero.
+ */
+int dora_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int w_dtype,
+                        const void* mean, const void* rstd, void* dx, void* d_weight, void* d_bias, void* workspace,
+                        size_t workspace_bytes, int64_t rows, int64_t cols, int act_dtype, void* stream);
+int dora_rms_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int w_dtype,
+                      const void* rstd, void* dx, void* d_weight, void* workspace, size_t workspace_bytes,
+                      int64_t rows, int64_t cols, int act_dtype, void* stream);
+
+/*
+ * Log probabilities of one given token a row of logits [rows x vocab] (row stride ld,
+ * unit column stride).  With x' = logits / temperature and L = log sum exp x':
+ *   logprobs = x'[target] - L, lse = L, entropy = -sum p log p (if entropy != NULL),
+ *   top_logprobs / top_indices [rows x top_k] = the largest x' - L and their columns,
+ *   in descending order, ties to the lower column (0 <= top_k <= 64, <= vocab).
+ * targets and top_indices are int64, the other outputs fp32.  A row whose target is
+ * ignore_index is not read and gives zeros (top_indices -1).  A target outside
+ * [0, vocab) gives a NaN log probability and sets DORA_ERR_INVALID_ARGUMENT in the device
+ * error word.  A row of -inf alone gives L = log probabilities = -inf and entropy 0;
+ * a row with a NaN or +inf gives NaN, and columns 0 .. top_k - 1.
+ */
+int dora_token_logprobs_fwd(const void* logits, int64_t ld, const void* targets, int64_t ignore_index,
+                            double temperature, void* logprobs, void* lse, void* entropy, int top_k,
+                            void* top_logprobs, void* top_indices, int64_t rows, int64_t vocab, int dtype,
+                            void* stream);
+
+/*
+ * Its gradient, from lse and entropy as the forward gave them and the gradients of
+ * logprobs, entropy and lse (fp32 [rows], each may be NULL for zero):
+ *   d_logits[j] = (g_logprobs (1[j = target] - p_j) - g_entropy p_j (log p_j + entropy)
+ *                  + g_lse p_j) / temperature
+ * in dtype with row stride ld_d.  d_logits may be logits itself (same stride).  Ignored
+ * rows and rows of -inf alone give zeros.
+ */
+int dora_token_logprobs_bwd(const void* logits, int64_t ld, const void* targets, int64_t ignore_index,
+                            double temperature, const void* lse, const void* entropy, const void* g_logprobs,
+                            const void* g_entropy, const void* g_lse, void* d_logits, int64_t ld_d, int64_t rows,
+                            int64_t vocab, int dtype, void* stream);
+
+/*
+ * One parameter of an AdamW step.  All arrays are contiguous, of numel elements in the
+ * same order.  exp_avg and exp_avg_sq are fp32, or codes of 8 bits with an fp32 scale for
+ * each 256 elements (exp_avg_scale, exp_avg_sq_scale: ceil(numel / 256) values).  master,
+ * for 16-bit parameters, is an fp32 copy that the step is taken on (NULL: none; all
+ * tensors of a call have one or none has).  key seeds the rounding of 8-bit exp_avg_sq.
+ */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* exp_avg_scale;
+  void* exp_avg_sq_scale;
+  void* master;
+  int64_t numel;
+  uint32_t key;
+  uint32_t reserved;
+} dora_adamw_tensor_t;
+
+/*
+ * AdamW on `count` parameters of one dtype (gradients have the same), updated in place:
+ *   m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in fp32.  `tensors` is host memory, read before the call returns.  state_bits 32 or 8:
+ * an 8-bit code holds a small floating-point number, times the block's scale (largest
+ * magnitude / 1.875): exp_avg sign, 4 exponent and 3 mantissa bits, exp_avg_sq 5 exponent
+ * and 3 mantissa bits; code 0 is zero, other codes 2^(c / 8 - bias) (1 + c % 8 / 8) with
+ * bias 15 (of the lower 7 bits) and 31.  exp_avg is rounded to nearest, exp_avg_sq up or
+ * down by bits hashed from key and the element's number.  A non-finite gradient makes
+ * the whole block's moments non-finite.
+ */
+int dora_adamw_step(const dora_adamw_tensor_t* tensors, int64_t count, int param_dtype, int state_bits, double lr,
+                    double beta1, double beta2, double eps, double weight_decay, int64_t step, void* stream);
+
+/* The fp32 values that numel 8-bit moments stand for (blocks of 256 from the start). */
+int dora_adamw_decode(const void* exp_avg_codes, const void* exp_avg_scale, const void* exp_avg_sq_codes,
+                      const void* exp_avg_sq_scale, void* exp_avg, void* exp_avg_sq, int64_t numel, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
