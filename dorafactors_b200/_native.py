@@ -525,11 +525,11 @@ ADAMW_TENSOR = [("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg_sq
                 ("exp_avg_sq_scale", "u8"), ("master", "u8"), ("numel", "i8"), ("key", "u4"), ("reserved", "u4")]
 
 
-def adamw_step(table, dtype: torch.dtype, state_bits: int, lr: float, betas, eps: float, weight_decay: float,
-               step: int, device: torch.device) -> None:
-    """``table``: a contiguous numpy array of ``ADAMW_TENSOR`` records."""
+def adamw_step(table: int, count: int, dtype: torch.dtype, state_bits: int, lr: float, betas, eps: float,
+               weight_decay: float, step: int, device: torch.device) -> None:
+    """``table``: the host address of ``count`` contiguous ``ADAMW_TENSOR`` records."""
     with on_device(device):
-        code = load_library().dora_adamw_step(table.ctypes.data, len(table), DTYPE_CODE[dtype], state_bits, lr,
+        code = load_library().dora_adamw_step(table, count, DTYPE_CODE[dtype], state_bits, lr,
                                               betas[0], betas[1], eps, weight_decay, step, _raw_stream(device))
     if code:
         check(code, "dora_adamw_step")

@@ -16,14 +16,19 @@ parameter at a multiple of 256 elements; ``state[p]`` has views of them.
 
 from __future__ import annotations
 
+import array
 import math
 
 import numpy as np
 import torch
+from torch.optim import optimizer as _base
 
 from . import _native
 
 BLOCK = 256  # elements that share a scale, and the granule of the flat buffers
+
+_data_ptr, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_numel, _device = torch.Tensor.numel, torch.Tensor.get_device
 
 
 class _Group:
@@ -65,13 +70,17 @@ class _Group:
             self.flat["master"] = zeros(self.numel, torch.float32)
 
         self.table = np.zeros(len(params), dtype=_native.ADAMW_TENSOR)
+        self.address = self.table.ctypes.data
         self.table["numel"] = sizes
         column = {"exp_avg_codes": "exp_avg", "exp_avg_sq_codes": "exp_avg_sq"}
         for name, buf in self.flat.items():
             per = 1 if name.endswith("_scale") else BLOCK
             self.table[column.get(name, name)] = buf.data_ptr() + starts[:-1] * (per * buf.element_size())
         self.index = np.arange(first, first + len(params), dtype=np.uint64)
-        self.strides = [p.stride() for p in params]
+        # What every step holds the tensors to, as lists that compare in one pass.
+        self.sizes, self.dtypes = sizes, [self.dtype] * len(params)
+        self.devices = [dev.index] * len(params)
+        self.states = [state[p] for p in params]
         for i, p in enumerate(params):
             st = state[p]
             st["step"] = 0
@@ -126,55 +135,75 @@ class AdamW(torch.optim.Optimizer):
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 8 or 32, got {group['state_bits']}")
 
-    @torch.no_grad()
     def step(self, closure=None):
+        # The base class wraps ``step`` for its hooks and a profiler range, which takes the host
+        # longer than a step of few tensors does; without hooks there is nothing to wrap.
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks
+                or getattr(_base, "_global_optimizer_pre_hooks", None)
+                or getattr(_base, "_global_optimizer_post_hooks", None)):
+            return _step_with_hooks(self, closure)
+        return self._step_all(closure)
+
+    step.hooked = True  # the base class wraps it otherwise
+
+    def _step_all(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step cannot be captured in a CUDA graph (its bias corrections are host numbers)")
         for group, g in zip(self.param_groups, self._groups):
+            self._check(group)
             self._step(group, g)
         return loss
 
     def _step(self, group: dict, g: _Group) -> None:
         params = g.params
         grads = [p.grad for p in params]
-        at = None
-        if any(x is None for x in grads):  # parameters that took no part in this step stay as they are
+        table, index, states = g.table, g.index, g.states
+        sizes, dtypes, devices = g.sizes, g.dtypes, g.devices
+        try:
+            grad_ptrs = list(map(_data_ptr, grads))
+        except TypeError:  # parameters without a gradient stay as they are
             at = [i for i, x in enumerate(grads) if x is not None]
             if not at:
                 return
-            params, grads = [params[i] for i in at], [grads[i] for i in at]
-        strides = g.strides if at is None else [g.strides[i] for i in at]
-        if [x.stride() for x in grads] != strides or [p.stride() for p in params] != strides:
-            if any(x.is_sparse for x in grads) or not all(p.is_contiguous() for p in params):
-                raise ValueError("AdamW: parameters must stay contiguous, and gradients dense")
-            grads = [x.contiguous() for x in grads]
-        if any(x.dtype is not g.dtype for x in grads) or any(p.dtype is not g.dtype for p in params):
-            raise ValueError(f"AdamW: parameters and gradients of this group must stay {g.dtype}")
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: a step cannot be captured in a CUDA graph (its bias corrections are host numbers)")
-        table = g.table if at is None else g.table[at]
-        table["param"] = [p.data_ptr() for p in params]
-        table["grad"] = [x.data_ptr() for x in grads]
-        self._check(group)
-        state = [self.state[p] for p in params]
-        steps = [st["step"] + 1 for st in state]
-        index = g.index if at is None else g.index[at]
+            table, index = table[at], index[at]
+            params, grads, states, sizes, dtypes, devices = ([of[i] for i in at] for of in (
+                params, grads, states, sizes, dtypes, devices))
+            grad_ptrs = None
+        if not all(map(_contiguous, grads)):
+            if any(x.layout is not torch.strided for x in grads):
+                raise ValueError("AdamW: gradients must be dense")
+            grads, grad_ptrs = [x.contiguous() for x in grads], None
+        if grad_ptrs is None:
+            grad_ptrs = list(map(_data_ptr, grads))
+        for of, what in ((params, "parameters"), (grads, "gradients")):
+            if list(map(_device, of)) != devices:
+                raise RuntimeError(f"AdamW: {what} must stay on {g.device}")
+            if [x.dtype for x in of] != dtypes or list(map(_numel, of)) != sizes:
+                raise ValueError(f"AdamW: {what} must keep their type ({g.dtype}) and size")
+        if not all(map(_contiguous, params)):
+            raise ValueError("AdamW: parameters must stay contiguous")
+        table["param"] = array.array("Q", map(_data_ptr, params))
+        table["grad"] = array.array("Q", grad_ptrs)
+        steps = [st["step"] for st in states]
         if steps.count(steps[0]) == len(steps):
-            self._launch(group, g, table, index, steps[0])
+            self._launch(group, g, table, index, steps[0] + 1)
         else:  # parameters that have seen different numbers of steps have their own corrections
             of = np.array(steps)
             for t in sorted(set(steps)):
-                self._launch(group, g, table[of == t], index[of == t], t)
-        for st, t in zip(state, steps):
-            st["step"] = t
+                self._launch(group, g, table[of == t], index[of == t], t + 1)
+        for st, t in zip(states, steps):
+            st["step"] = t + 1
 
     def _launch(self, group: dict, g: _Group, table, index, step: int) -> None:
         if g.bits == 8:
             key = (self.seed + step * 0x9E3779B1) & 0xFFFFFFFF
             table["key"] = (np.uint64(key) + index * np.uint64(0xC2B2AE35)) & np.uint64(0xFFFFFFFF)
-        _native.adamw_step(table, g.dtype, g.bits, float(group["lr"]), group["betas"], group["eps"],
+        address = g.address if table is g.table else table.ctypes.data
+        _native.adamw_step(address, len(table), g.dtype, g.bits, float(group["lr"]), group["betas"], group["eps"],
                            group["weight_decay"], step, g.device)
 
     @torch.no_grad()
@@ -233,3 +262,6 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state: dict) -> None:
         raise NotImplementedError("AdamW: pickle its state_dict(), not the optimizer")
+
+
+_step_with_hooks = torch.optim.Optimizer.profile_hook_step(AdamW._step_all)
