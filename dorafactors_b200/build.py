@@ -24,7 +24,7 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libdora_b200.so")
 SOURCES = ["capi.cu", "compose.cu", "compose_ch.cu", "backward.cu", "norm_simt.cu", "norm_tc.cu", "norm_tc2.cu", "norm_sk.cu", "norm_sk2.cu", "norm.cu", "shard.cu", "peer.cu", "layernorm.cu", "logprobs.cu", "adamw.cu", "selftest.cu"]
-HEADERS = ["dora_common.cuh", "norm_internal.cuh", "tc_common.cuh"]
+HEADERS = ["dora_common.cuh", "pair.cuh", "norm_internal.cuh", "tc_common.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-rdc=true", "--expt-relaxed-constexpr"]
 

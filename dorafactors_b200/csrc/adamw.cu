@@ -19,7 +19,7 @@
 #include <cfloat>
 #include <type_traits>
 
-#include "dora_common.cuh"
+#include "pair.cuh"
 
 namespace dora {
 namespace {
@@ -86,35 +86,6 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int n, bool vec, uint64_
   else
     for (int i = 0; i < n; ++i) p[i] = uint8_t(c >> (8 * i));
 }
-
-// Two fp32 numbers in one instruction, each rounded like its scalar form.
-struct Two {
-  float a, b;
-};
-__device__ __forceinline__ unsigned long long bits2(Two x) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x.a), "f"(x.b));
-  return r;
-}
-__device__ __forceinline__ Two two(unsigned long long r) {
-  Two x;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x.a), "=f"(x.b) : "l"(r));
-  return x;
-}
-__device__ __forceinline__ Two mul2(Two x, Two y) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)));
-  return two(r);
-}
-__device__ __forceinline__ Two fma2(Two x, Two y, Two z) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)), "l"(bits2(z)));
-  return two(r);
-}
-__device__ __forceinline__ Two both(float x) { return Two{x, x}; }
-// A sum as a product with 1: the compiler joins a packed product and a packed sum into one FMA,
-// with one rounding where the moments' definition has two.
-__device__ __forceinline__ Two add2(Two x, Two y, Two one) { return fma2(x, one, y); }
 
 // The work on codes is what bounds the 8-bit step (the ALU pipe: shifts, logic, minima), so it is laid
 // out in few such operations.  A code is bits 27..20 of the scaled number's fp32 pattern, the sign in
@@ -221,8 +192,8 @@ __device__ __forceinline__ void step_block(const dora_adamw_tensor_t& d, const S
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const Two g{gf[2 * j], gf[2 * j + 1]};
-    m[j] = add2(mul2(m[j], both(s.b1)), mul2(g, both(s.omb1)), both(s.one));
-    v[j] = add2(mul2(v[j], both(s.b2)), mul2(mul2(g, g), both(s.omb2)), both(s.one));
+    m[j] = add2_apart(mul2(m[j], both(s.b1)), mul2(g, both(s.omb1)), both(s.one));
+    v[j] = add2_apart(mul2(v[j], both(s.b2)), mul2(mul2(g, g), both(s.omb2)), both(s.one));
     Two q;
     if constexpr (k8) {
       // Two units in the last place of the step are far below the codes' own rounding.  2^-126 is
@@ -334,14 +305,6 @@ template <int kWords, int kGradWords> struct Stage {
   uint4 g[kGradWords][32], p[kWords][32];
   uint2 m[32], v[32];
 };
-__device__ __forceinline__ void copy_async16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from)
-               : "memory");
-}
-__device__ __forceinline__ void copy_async8(void* to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from)
-               : "memory");
-}
 template <typename T> __device__ __forceinline__ void unstage(const uint4 (*w)[32], int lane, float (&f)[8]) {
   if constexpr (sizeof(T) == 4) {
     float lo[4], hi[4];
@@ -388,13 +351,13 @@ adamw_kernel(const __grid_constant__ Table<N> tab, const __grid_constant__ Scala
         Staged& to = st[k % (kAhead + 1)];
         const int64_t o = int64_t(k) * kStride;
 #pragma unroll
-        for (int w = 0; w < kGradWords; ++w) copy_async16(&to.g[w][lane], g + o + w * 4);
+        for (int w = 0; w < kGradWords; ++w) copy_async16(shared_addr(&to.g[w][lane]), g + o + w * 4);
 #pragma unroll
-        for (int w = 0; w < kWords; ++w) copy_async16(&to.p[w][lane], p + o + w * 4);
-        copy_async8(&to.m[lane], mc + o);
-        copy_async8(&to.v[lane], vc + o);
+        for (int w = 0; w < kWords; ++w) copy_async16(shared_addr(&to.p[w][lane]), p + o + w * 4);
+        copy_async8(shared_addr(&to.m[lane]), mc + o);
+        copy_async8(shared_addr(&to.v[lane]), vc + o);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      copies_commit();
     };
     const float *ms = static_cast<const float*>(d.exp_avg_scale), *vs = static_cast<const float*>(d.exp_avg_sq_scale);
     float ms0 = 0.f, vs0 = 0.f;
@@ -404,7 +367,7 @@ adamw_kernel(const __grid_constant__ Table<N> tab, const __grid_constant__ Scala
 #pragma unroll 1
     for (int k = 0; k < full; ++k, b += kStride) {
       fetch(k + kAhead);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+      copies_done<kAhead>();
       const Staged& from = st[k % (kAhead + 1)];
       Lane<true> x;
       unstage<TP>(from.g, lane, x.g);

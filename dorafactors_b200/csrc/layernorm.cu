@@ -8,31 +8,557 @@
 //
 // Statistics, row sums and the column sums are fp32 in a fixed order (no atomics), so
 // results do not change from call to call; every output is rounded once.
-#include "dora_common.cuh"
+#include <type_traits>
+
+#include "pair.cuh"
 
 namespace dora {
 namespace {
 
-constexpr int kT = 256;  // threads of the row kernels
+constexpr int kT = 256;       // threads of the kernels for any width
+constexpr int kFwdFill = 768, kBwdFill = 512;
 
-// Sum over the CTA, in every thread; the same tree each time.  `red` holds one value a warp.
+// ---------------------------------------------------------------------------
+// A row and the threads that share it.  `tpr` threads hold a row: up to 32 (a power of
+// two) of a warp, whose CTA then works on several rows, or whole warps of a CTA.
+// ---------------------------------------------------------------------------
+struct Shape {
+  int tpr, threads, groups;  // threads a row and a CTA, rows a CTA works on at a time
+};
+Shape share_row(int64_t units, int per, int small_cta) {
+  Shape s;
+  const int64_t need = (units + per - 1) / per;
+  if (need > 32) {
+    s.tpr = s.threads = int((need + 31) / 32 * 32);
+    s.groups = 1;
+  } else {
+    s.tpr = 1;
+    while (s.tpr < need) s.tpr *= 2;
+    s.threads = small_cta;
+    s.groups = small_cta / s.tpr;
+  }
+  return s;
+}
+
+// Sums over the threads of a row, in every one of them; the same tree each time.  kMost: threads of the
+// CTA, all of one row, or 128 for rows inside a warp.  One barrier a call: `red` alternates between two
+// buffers, and a buffer is written again only after the barrier of the call in between.
+template <int kMost, int kValues> struct RowSum {
+  static constexpr bool kWide = kMost > 128;
+  static constexpr int kWarps = kWide ? kMost / 32 : 1;
+  float4 (*red)[kValues][kWarps / 4 + 1];  // [2] in shared memory: a value a warp, zero for warps that are not there
+  int tpr, turn;
+  __device__ RowSum(float4 (*r)[kValues][kWarps / 4 + 1], int tpr_) : red(r), tpr(tpr_), turn(0) {
+    if constexpr (kWide) {
+      float* f = reinterpret_cast<float*>(red);
+      for (int i = threadIdx.x; i < 2 * kValues * (kWarps / 4 + 1) * 4; i += blockDim.x) f[i] = 0.f;
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void operator()(float (&v)[kValues]) {
+    if constexpr (!kWide) {
+      for (int o = tpr / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) reinterpret_cast<float*>(red[turn][i])[threadIdx.x / 32] = v[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) {
+        Two t = both(0.f);
+#pragma unroll
+        for (int j = 0; j < kWarps / 4; ++j) {
+          const float4 q = red[turn][i][j];
+          t = add2(t, add2(Two{q.x, q.y}, Two{q.z, q.w}));
+        }
+        v[i] = t.a + t.b;
+      }
+      turn ^= 1;
+    }
+  }
+};
+#define DORA_ROW_SUM(name, most, values)                                                  \
+  __shared__ float4 name##_red[2][values][RowSum<most, values>::kWarps / 4 + 1];          \
+  RowSum<most, values> name(name##_red, tpr)
+
+// A unit (16-byte vector of T) of the weight or bias at column c, as pairs.
+template <typename T, typename TW>
+__device__ __forceinline__ void load_param(const void* w, int64_t c, Two (&f)[Pairs<T>::N]) {
+  if constexpr (sizeof(TW) == 4) {
+#pragma unroll
+    for (int i = 0; i < Pairs<T>::N; i += 2) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + c + 2 * i));
+      f[i] = Two{q.x, q.y}, f[i + 1] = Two{q.z, q.w};
+    }
+  } else {
+    Pairs<T>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w) + c)), f);
+  }
+}
+// The same where type and presence (`none` instead) are known at run time only.
+template <typename T>
+__device__ __forceinline__ void load_param(const void* w, bool f32, int64_t c, float none, Two (&f)[Pairs<T>::N]) {
+  if (!w) {
+#pragma unroll
+    for (int i = 0; i < Pairs<T>::N; ++i) f[i] = both(none);
+  } else if (f32) {
+    load_param<T, float>(w, c, f);
+  } else {
+    load_param<T, T>(w, c, f);
+  }
+}
+template <typename T> __device__ __forceinline__ float param(const void* w, bool f32, int64_t c, float none) {
+  if (!w) return none;
+  return f32 ? __ldg(static_cast<const float*>(w) + c) : to_f32(static_cast<const T*>(w)[c]);
+}
+
+// ---------------------------------------------------------------------------
+// Rows of 16-byte units.  A CTA walks down the rows; a thread keeps the same PER units
+// of every row (and their weights in registers) and has the next S - 1 rows' units on
+// their way through shared memory, which keeps HBM busy across the barriers of a row's
+// sums.  A thread reads back only what it has copied itself.
+// ---------------------------------------------------------------------------
+struct Walk {  // this thread's part of the rows
+  int t, group;        // its number among the row's threads, and the row's among the CTA's
+  int64_t first, step; // row it starts with and distance to the next
+  int64_t mine, rounds; // its rows, and rounds of the CTA
+};
+__device__ __forceinline__ Walk walk(int64_t rows, int tpr, int groups) {
+  Walk w;
+  w.t = groups > 1 ? threadIdx.x & (tpr - 1) : threadIdx.x;
+  w.group = groups > 1 ? threadIdx.x / tpr : 0;
+  w.step = int64_t(gridDim.x) * groups;
+  const int64_t r0 = int64_t(blockIdx.x) * groups;
+  w.first = r0 + w.group;
+  w.rounds = r0 < rows ? (rows - r0 + w.step - 1) / w.step : 0;
+  w.mine = w.first < rows ? (rows - w.first + w.step - 1) / w.step : 0;
+  return w;
+}
+
+// Forward: the variance is taken around the mean, from the registers.
+// kParams: 0 none, 1 a weight, 2 a weight and a bias, of type TW; they come from L1 for each row.
+template <typename TA, typename TW, bool kRms, int kParams, int PER, int S, int kMax>
+__global__ void __launch_bounds__(kMax, kFwdFill / kMax)
+ln_fwd_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, float eps, TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
+              int cols, int tpr, int groups) {
+  using P = Pairs<TA>;
+  constexpr int N = P::N, V = 2 * N;
+  extern __shared__ uint4 ring[];  // [S][PER][threads]
+  DORA_ROW_SUM(sum, kMax, 1);
+  const Walk at = walk(rows, tpr, groups);
+  const float inv = 1.0f / float(cols);
+  bool has[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) has[p] = p == 0 || (p * tpr + at.t) * V < cols;  // every thread has a first unit
+  const TA* from = x + at.first * ldx + at.t * V;
+  TA* to = y + at.first * cols + at.t * V;
+  const uint32_t slots = shared_addr(ring + threadIdx.x), part = blockDim.x * 16;
+  int64_t fetched = 0;
+  int into = 0;
+  auto fetch = [&] {
+    if (fetched < at.mine) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p)
+        if (has[p]) copy_async16(slots + (into * PER + p) * part, from + p * tpr * V);
+      from += at.step * ldx;
+      ++fetched;
+    }
+    copies_commit();
+    into = into == S - 1 ? 0 : into + 1;
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch();
+  int s = 0;
+  for (int64_t k = 0; k < at.rounds; ++k) {
+    fetch();
+    copies_done<S - 1>();
+    const bool live = kMax > 128 || k < at.mine;  // rows inside a warp: all its threads take part in the sums
+    Two f[PER][N];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      if (live && has[p]) P::unpack(ring[(s * PER + p) * blockDim.x + threadIdx.x], f[p]);
+      else
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[p][i] = both(0.f);
+    }
+    s = s == S - 1 ? 0 : s + 1;
+    float mu[1] = {0.f}, var[1];
+    if constexpr (!kRms) {
+      Two a = both(0.f);
+#pragma unroll
+      for (int p = 0; p < PER; ++p)
+#pragma unroll
+        for (int i = 0; i < N; ++i) a = add2(a, f[p][i]);
+      mu[0] = a.a + a.b;
+      sum(mu);
+      mu[0] *= inv;
+    }
+    Two q = both(0.f);
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (has[p]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if constexpr (!kRms) f[p][i] = add2(f[p][i], both(-mu[0]));
+          q = fma2(f[p][i], f[p][i], q);
+        }
+      }
+    var[0] = q.a + q.b;
+    sum(var);
+    const float rs = rsqrtf(var[0] * inv + eps);
+    if (live) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p)
+        if (has[p]) {
+          Two o[N], v[N];
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[i] = mul2(f[p][i], both(rs));
+          if constexpr (kParams > 0) {
+            load_param<TA, TW>(w, (p * tpr + at.t) * V, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] = mul2(o[i], v[i]);
+          }
+          if constexpr (kParams > 1) {
+            load_param<TA, TW>(b, (p * tpr + at.t) * V, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] = add2(o[i], v[i]);
+          }
+          st_stream(to + p * tpr * V, P::pack(o));
+        }
+      if (at.t == 0) {
+        const int64_t r = at.first + k * at.step;
+        if (!kRms && mean) mean[r] = mu[0];
+        if (rstd) rstd[r] = rs;
+      }
+    }
+    to += at.step * cols;
+  }
+}
+
+// Backward: one pass over dy and x, with the columns' sums for d_weight and d_bias in
+// registers; they cost no traffic but one partial row a CTA.
+template <typename TA, bool kRms, int PER, int S, int kMax, bool kCols>
+__global__ void __launch_bounds__(kMax)
+ln_bwd_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
+              const void* __restrict__ w, bool f32, const float* __restrict__ mean, const float* __restrict__ rstd,
+              TA* __restrict__ dx, float* __restrict__ partial, int64_t rows, int cols, int tpr, int groups,
+              float one_) {
+  using P = Pairs<TA>;
+  constexpr int N = P::N, V = 2 * N;
+  constexpr bool kHold = kMax <= 512;  // registers for the weight
+  extern __shared__ uint4 ring[];  // [S][PER][2][threads]
+  constexpr int kSums = kRms ? 1 : 2;
+  DORA_ROW_SUM(sum, kMax, kSums);
+  const Walk at = walk(rows, tpr, groups);
+  const float inv = 1.0f / float(cols);
+  const Two one = both(one_);
+  bool has[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) has[p] = p == 0 || (p * tpr + at.t) * V < cols;  // every thread has a first unit
+  const TA *dfrom = dy + at.first * lddy + at.t * V, *xfrom = x + at.first * ldx + at.t * V;
+  TA* to = dx + at.first * cols + at.t * V;
+  const uint32_t slots = shared_addr(ring + threadIdx.x), part = blockDim.x * 16;
+  int64_t fetched = 0;
+  int into = 0;
+  auto fetch = [&] {
+    if (fetched < at.mine) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p)
+        if (has[p]) {
+          copy_async16(slots + (into * PER + p) * 2 * part, dfrom + p * tpr * V);
+          copy_async16(slots + (into * PER + p) * 2 * part + part, xfrom + p * tpr * V);
+        }
+      dfrom += at.step * lddy;
+      xfrom += at.step * ldx;
+      ++fetched;
+    }
+    copies_commit();
+    into = into == S - 1 ? 0 : into + 1;
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch();
+  Two wf[kHold ? PER : 1][N], dw[kCols ? PER : 1][N], db[kCols && !kRms ? PER : 1][N];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    if (kHold && has[p]) load_param<TA>(w, f32, (p * tpr + at.t) * V, 1.f, wf[p]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (kCols) dw[p][i] = both(0.f);
+      if constexpr (kCols && !kRms) db[p][i] = both(0.f);
+    }
+  }
+  const float *mnext = kRms ? nullptr : mean + at.first, *rnext = rstd + at.first;
+  float mu1 = 0.f, rs1 = 0.f;  // of the next row
+  if (at.mine) {
+    if constexpr (!kRms) mu1 = *mnext;
+    rs1 = *rnext;
+  }
+  int s = 0;
+  for (int64_t k = 0; k < at.rounds; ++k) {
+    const float mu = mu1, rs = rs1;
+    if (k + 1 < at.mine) {
+      if constexpr (!kRms) mu1 = *(mnext += at.step);
+      rs1 = *(rnext += at.step);
+    }
+    fetch();
+    copies_done<S - 1>();
+    const bool live = kMax > 128 || k < at.mine;
+    uint4 dq[PER], xq[PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      dq[p] = ring[(s * PER + p) * 2 * blockDim.x + threadIdx.x];
+      xq[p] = ring[((s * PER + p) * 2 + 1) * blockDim.x + threadIdx.x];
+    }
+    s = s == S - 1 ? 0 : s + 1;
+    auto take = [&](int p, Two (&d)[N], Two (&h)[N], Two (&a)[N]) {  // dy, xh and dy w
+      P::unpack(dq[p], d);
+      P::unpack(xq[p], h);
+      if constexpr (!kHold) load_param<TA>(w, f32, (p * tpr + at.t) * V, 1.f, a);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        a[i] = mul2(d[i], kHold ? wf[p][i] : a[i]);
+        if constexpr (!kRms) h[i] = add2(h[i], both(-mu));
+        h[i] = mul2(h[i], both(rs));
+      }
+    };
+    Two s0 = both(0.f), s1 = both(0.f);
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (live && has[p]) {
+        Two d[N], h[N], a[N];
+        take(p, d, h, a);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if constexpr (!kRms) s0 = add2_apart(a[i], s0, one);
+          s1 = fma2(a[i], h[i], s1);
+          if constexpr (kCols) dw[p][i] = fma2(d[i], h[i], dw[p][i]);
+          if constexpr (kCols && !kRms) db[p][i] = add2(db[p][i], d[i]);
+        }
+      }
+    if (dx) {  // the same for all threads
+      float c[kSums];
+      c[0] = s1.a + s1.b;
+      if constexpr (!kRms) c[1] = s0.a + s0.b;
+      sum(c);
+      const Two c0 = both(kRms ? 0.f : -c[kSums - 1] * inv), c1 = both(-c[0] * inv);
+#pragma unroll
+      for (int p = 0; p < PER; ++p)
+        if (live && has[p]) {
+          Two d[N], h[N], a[N];
+          take(p, d, h, a);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if constexpr (!kRms) a[i] = add2_apart(a[i], c0, one);
+            a[i] = mul2(fma2(h[i], c1, a[i]), both(rs));
+          }
+          st_stream(to + p * tpr * V, P::pack(a));
+        }
+      to += at.step * cols;
+    }
+  }
+  if constexpr (kCols) {
+    copies_done<0>();
+    float* out = partial + int64_t(blockIdx.x) * 2 * cols;
+    float* acc = groups > 1 ? reinterpret_cast<float*>(ring) : out;  // the groups add up in shared memory, one by one
+    for (int g = 0; g < groups; ++g) {
+      if (groups > 1) __syncthreads();
+      if (at.group == g)
+#pragma unroll
+        for (int p = 0; p < PER; ++p)
+          if (has[p]) {
+            float2* o = reinterpret_cast<float2*>(acc + (p * tpr + at.t) * V);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const float2 q = g ? o[i] : make_float2(0.f, 0.f);
+              o[i] = make_float2(dw[p][i].a + q.x, dw[p][i].b + q.y);
+              if constexpr (!kRms) {
+                float2* ob = o + i + cols / 2;
+                const float2 v = g ? *ob : make_float2(0.f, 0.f);
+                *ob = make_float2(db[p][i].a + v.x, db[p][i].b + v.y);
+              }
+            }
+          }
+    }
+    if (groups > 1) {
+      __syncthreads();
+      for (int c = threadIdx.x; c < (kRms ? 1 : 2) * cols; c += blockDim.x) out[c] = acc[c];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows that start or end off a 16-byte boundary: the same by elements, read
+// straight from global memory (the backward's second time from L2).
+// ---------------------------------------------------------------------------
+template <typename TA, bool kRms, int PER, int kMax>
+__global__ void __launch_bounds__(kMax)
+ln_fwd_element_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b,
+                      bool f32, float eps, TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
+                      int64_t rows, int cols, int tpr, int groups) {
+  DORA_ROW_SUM(sum, kMax, 1);
+  const Walk at = walk(rows, tpr, groups);
+  const float inv = 1.0f / float(cols);
+  for (int64_t k = 0; k < at.rounds; ++k) {
+    const bool live = k < at.mine;
+    const int64_t r = at.first + k * at.step;
+    const TA* xr = x + r * ldx;
+    float f[PER];
+    float a = 0.f;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int c = p * tpr + at.t;
+      f[p] = live && c < cols ? to_f32(xr[c]) : 0.f;
+      a += f[p];
+    }
+    float one[1] = {a};
+    if constexpr (!kRms) sum(one);
+    const float mu = kRms ? 0.f : one[0] * inv;
+    one[0] = 0.f;
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (p * tpr + at.t < cols) {
+        f[p] -= mu;
+        one[0] = fmaf(f[p], f[p], one[0]);
+      }
+    sum(one);
+    const float rs = rsqrtf(one[0] * inv + eps);
+    if (!live) continue;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int c = p * tpr + at.t;
+      if (c < cols) y[r * cols + c] = from_f32<TA>(fmaf(f[p] * rs, param<TA>(w, f32, c, 1.f), param<TA>(b, f32, c, 0.f)));
+    }
+    if (at.t == 0) {
+      if (!kRms && mean) mean[r] = mu;
+      if (rstd) rstd[r] = rs;
+    }
+  }
+}
+
+template <typename TA, bool kRms, int PER, int kMax, bool kCols>
+__global__ void __launch_bounds__(kMax)
+ln_bwd_element_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
+                      const void* __restrict__ w, bool f32, const float* __restrict__ mean,
+                      const float* __restrict__ rstd, TA* __restrict__ dx, float* __restrict__ partial, int64_t rows,
+                      int cols, int tpr, int groups) {
+  extern __shared__ float joined[];  // [2][cols] where a CTA works on several rows
+  DORA_ROW_SUM(sum, kMax, 2);
+  const Walk at = walk(rows, tpr, groups);
+  const float inv = 1.0f / float(cols);
+  float dw[kCols ? PER : 1] = {}, db[kCols && !kRms ? PER : 1] = {};
+  for (int64_t k = 0; k < at.rounds; ++k) {
+    const bool live = k < at.mine;
+    const int64_t r = at.first + k * at.step;
+    const TA *xr = x + r * ldx, *dr = dy + r * lddy;
+    float mu = 0.f, rs = 0.f;
+    if (live) {
+      if constexpr (!kRms) mu = mean[r];
+      rs = rstd[r];
+    }
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int c = p * tpr + at.t;
+      if (live && c < cols) {
+        const float d = to_f32(dr[c]), h = (to_f32(xr[c]) - mu) * rs, a = __fmul_rn(d, param<TA>(w, f32, c, 1.f));
+        s0 += a;
+        s1 = fmaf(a, h, s1);
+        if constexpr (kCols) dw[p] = fmaf(d, h, dw[p]);
+        if constexpr (kCols && !kRms) db[p] += d;
+      }
+    }
+    if (dx) {  // the same for all threads
+      float c01[2] = {s0, s1};
+      sum(c01);
+      const float c0 = kRms ? 0.f : c01[0] * inv, c1 = c01[1] * inv;
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int c = p * tpr + at.t;
+        if (live && c < cols) {
+          const float a = __fmul_rn(to_f32(dr[c]), param<TA>(w, f32, c, 1.f));
+          dx[r * cols + c] = from_f32<TA>((a - c0 - (to_f32(xr[c]) - mu) * rs * c1) * rs);
+        }
+      }
+    }
+  }
+  if constexpr (kCols) {
+    float* out = partial + int64_t(blockIdx.x) * 2 * cols;
+    float* acc = groups > 1 ? joined : out;
+    for (int g = 0; g < groups; ++g) {
+      if (groups > 1) __syncthreads();
+      if (at.group == g)
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+          const int c = p * tpr + at.t;
+          if (c < cols) {
+            acc[c] = dw[p] + (g ? acc[c] : 0.f);
+            if constexpr (!kRms) acc[cols + c] = db[p] + (g ? acc[cols + c] : 0.f);
+          }
+        }
+    }
+    if (groups > 1) {
+      __syncthreads();
+      for (int c = threadIdx.x; c < (kRms ? 1 : 2) * cols; c += blockDim.x) out[c] = acc[c];
+    }
+  }
+}
+
+// Sums the Z partial rows of dw (and db, `halves` 2): a CTA 32 columns, 8 slices of Z, joined in order.
+template <typename TW>
+__global__ void __launch_bounds__(kT)
+ln_col_finish_kernel(const float* __restrict__ partial, int Z, TW* __restrict__ dw, TW* __restrict__ db, int cols) {
+  __shared__ float part[8][33];
+  const int half = blockIdx.y;
+  TW* out = half ? db : dw;
+  if (!out) return;
+  const int64_t c = int64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+  const int slice = threadIdx.x / 32;
+  float a = 0.f;
+  if (c < cols) {
+    const float* p = partial + int64_t(half) * cols + c;
+    const int z1 = Z * (slice + 1) / 8;
+    int z = Z * slice / 8;
+    for (; z + 4 <= z1; z += 4) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __ldcg(p + int64_t(z + i) * 2 * cols);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a += v[i];
+    }
+    for (; z < z1; ++z) a += __ldcg(p + int64_t(z) * 2 * cols);
+  }
+  part[slice][threadIdx.x & 31] = a;
+  __syncthreads();
+  if (slice == 0 && c < cols) {
+    for (int i = 1; i < 8; ++i) a += part[i][threadIdx.x & 31];
+    out[c] = from_f32<TW>(a);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows wider than the kernels above hold: one CTA a row, which is read again for
+// each sum (from L2 after the first time).
+// ---------------------------------------------------------------------------
 __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int warps = blockDim.x / 32;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = v;
   __syncthreads();
   float t = 0.f;
-  for (int w = 0; w < warps; ++w) t += red[w];
+  for (int w = 0; w < kT / 32; ++w) t += red[w];
   __syncthreads();
   return t;
 }
-
-// One CTA a row, any width and alignment; the row is read three times (from L2 after the first).
-template <typename TA, typename TW, bool kRms>
+template <typename TA, bool kRms>
 __global__ void __launch_bounds__(kT)
-ln_fwd_any_kernel(const TA* __restrict__ x, int64_t ldx, const TW* __restrict__ w, const TW* __restrict__ b, float eps,
-                  TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t rows, int64_t cols) {
+ln_fwd_wide_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b,
+                   bool f32, float eps, TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
+                   int64_t rows, int64_t cols) {
   __shared__ float red[kT / 32];
   const float inv = 1.0f / float(cols);
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -49,12 +575,8 @@ ln_fwd_any_kernel(const TA* __restrict__ x, int64_t ldx, const TW* __restrict__ 
       q = fmaf(d, d, q);
     }
     const float rs = rsqrtf(block_sum(q, red) * inv + eps);
-    for (int64_t c = threadIdx.x; c < cols; c += kT) {
-      float v = (to_f32(xr[c]) - mu) * rs;
-      if (w) v *= to_f32(w[c]);
-      if (b) v += to_f32(b[c]);
-      y[r * cols + c] = from_f32<TA>(v);
-    }
+    for (int64_t c = threadIdx.x; c < cols; c += kT)
+      y[r * cols + c] = from_f32<TA>(fmaf((to_f32(xr[c]) - mu) * rs, param<TA>(w, f32, c, 1.f), param<TA>(b, f32, c, 0.f)));
     if (threadIdx.x == 0) {
       if (!kRms && mean) mean[r] = mu;
       if (rstd) rstd[r] = rs;
@@ -62,11 +584,11 @@ ln_fwd_any_kernel(const TA* __restrict__ x, int64_t ldx, const TW* __restrict__ 
   }
 }
 
-template <typename TA, typename TW, bool kRms>
+template <typename TA, bool kRms>
 __global__ void __launch_bounds__(kT)
-ln_bwd_any_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
-                  const TW* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
-                  TA* __restrict__ dx, int64_t rows, int64_t cols) {
+ln_bwd_wide_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
+                   const void* __restrict__ w, bool f32, const float* __restrict__ mean,
+                   const float* __restrict__ rstd, TA* __restrict__ dx, int64_t rows, int64_t cols) {
   __shared__ float red[kT / 32];
   const float inv = 1.0f / float(cols);
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -74,94 +596,199 @@ ln_bwd_any_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict_
     const float mu = kRms ? 0.f : mean[r], rs = rstd[r];
     float s0 = 0.f, s1 = 0.f;
     for (int64_t c = threadIdx.x; c < cols; c += kT) {
-      const float a = __fmul_rn(to_f32(dr[c]), w ? to_f32(w[c]) : 1.0f);
+      const float a = __fmul_rn(to_f32(dr[c]), param<TA>(w, f32, c, 1.f));
       s0 += a;
       s1 = fmaf(a, (to_f32(xr[c]) - mu) * rs, s1);
     }
     const float c0 = kRms ? 0.f : block_sum(s0, red) * inv;
     const float c1 = block_sum(s1, red) * inv;
     for (int64_t c = threadIdx.x; c < cols; c += kT) {
-      const float a = __fmul_rn(to_f32(dr[c]), w ? to_f32(w[c]) : 1.0f);
-      const float xh = (to_f32(xr[c]) - mu) * rs;
-      dx[r * cols + c] = from_f32<TA>((a - c0 - xh * c1) * rs);
+      const float a = __fmul_rn(to_f32(dr[c]), param<TA>(w, f32, c, 1.f));
+      dx[r * cols + c] = from_f32<TA>((a - c0 - (to_f32(xr[c]) - mu) * rs * c1) * rs);
     }
   }
 }
 
-// Column sums over one slab of rows: partial[z][0][c] of dy * xh, partial[z][1][c] of dy.
+// Column sums of one slab of rows.
 template <typename TA, bool kRms>
 __global__ void __launch_bounds__(kT)
-ln_col_any_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
-                  const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ partial,
-                  int64_t rows, int64_t cols) {
+ln_col_wide_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
+                   const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ partial,
+                   int64_t rows, int64_t cols) {
   const int64_t c = int64_t(blockIdx.x) * kT + threadIdx.x;
   if (c >= cols) return;
   const int64_t z = blockIdx.y, Z = gridDim.y;
   float dw = 0.f, db = 0.f;
   for (int64_t r = rows * z / Z; r < rows * (z + 1) / Z; ++r) {
     const float d = to_f32(dy[r * lddy + c]);
-    const float xh = (to_f32(x[r * ldx + c]) - (kRms ? 0.f : mean[r])) * rstd[r];
-    dw = fmaf(d, xh, dw);
+    dw = fmaf(d, (to_f32(x[r * ldx + c]) - (kRms ? 0.f : mean[r])) * rstd[r], dw);
     db += d;
   }
   partial[(2 * z) * cols + c] = dw;
-  partial[(2 * z + 1) * cols + c] = db;
+  if (!kRms) partial[(2 * z + 1) * cols + c] = db;
 }
 
-template <typename TW>
-__global__ void __launch_bounds__(kT)
-ln_col_finish_kernel(const float* __restrict__ partial, int Z, TW* __restrict__ dw, TW* __restrict__ db, int64_t cols) {
-  const int64_t c = int64_t(blockIdx.x) * kT + threadIdx.x;
-  if (c >= cols) return;
-  float a = 0.f, b = 0.f;
-  for (int64_t z = 0; z < Z; ++z) {
-    a += partial[(2 * z) * cols + c];
-    b += partial[(2 * z + 1) * cols + c];
-  }
-  if (dw) dw[c] = from_f32<TW>(a);
-  if (db) db[c] = from_f32<TW>(b);
-}
-
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
 unsigned row_grid(int64_t rows) { return unsigned(rows < (1 << 20) ? rows : (1 << 20)); }
 
-int col_slabs(int64_t rows, int64_t cols) {
+// How the threads of the row kernels share rows of `units` (16-byte vectors, or elements).
+struct Plan {
+  int per, most;  // units a thread holds, threads a CTA has at most; per 0: rows too wide
+  Shape shape;
+  int64_t ctas;
+};
+// `fill`: threads that an SM's registers hold, 64 of them a thread in the forward and 128 in the backward.  More
+// CTAs than fill the GPU would only divide the walk down the rows, and multiply the partial sums.
+Plan plan_rows(int64_t rows, int64_t units, bool vec, bool fwd) {
+  Plan p;
+  const int fill = fwd ? kFwdFill : kBwdFill;
+  if (vec && fwd) p.per = units <= 768 * 4 ? 4 : 0;
+  else p.per = vec ? (units <= 2048 ? 2 : 0) : units <= 2048 ? 4 : units <= 8192 ? 16 : 0;
+  if (!p.per) return p;
+  p.shape = share_row(units, p.per, 128);
+  if (vec && fwd) p.most = p.shape.groups > 1 ? 128 : p.shape.threads > 256 ? 768 : 256;
+  else p.most = p.shape.groups > 1 ? 128 : vec && units > 1024 ? 1024 : 512;
+  const int64_t held = int64_t(num_sms()) * (fill > p.shape.threads ? fill / p.shape.threads : 1);
+  const int64_t need = (rows + p.shape.groups - 1) / p.shape.groups;
+  p.ctas = need < 1 ? 1 : need < held ? need : held;
+  return p;
+}
+
+template <typename K> int allow_shared(K kernel, size_t bytes) {
+  if (bytes <= 40 * 1024) return DORA_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  return e == cudaSuccess ? DORA_OK : set_cuda_error(e);
+}
+
+template <typename TA, bool kRms>
+int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, bool f32, float eps, void* y, float* mean,
+               float* rstd, int64_t rows, int64_t cols, cudaStream_t st) {
+  constexpr int V = Vec16<TA>::N;
+  const bool vec = cols % V == 0 && ldx % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
+  const Plan p = plan_rows(rows, vec ? cols / V : cols, vec, true);
+  auto X = static_cast<const TA*>(x);
+  auto Y = static_cast<TA*>(y);
+  if (p.per && vec && (w || !b)) {
+    auto go = [&](auto kernel, int S) {
+      const size_t smem = size_t(S) * p.per * p.shape.threads * 16;
+      const int e = allow_shared(kernel, smem);
+      if (e) return e;
+      kernel<<<unsigned(p.ctas), p.shape.threads, smem, st>>>(X, ldx, w, b, eps, Y, mean, rstd, rows, int(cols),
+                                                              p.shape.tpr, p.shape.groups);
+      return check_launch();
+    };
+    auto sized = [&](auto tw, auto kind) {
+      using TW = decltype(tw);
+      constexpr int K = decltype(kind)::value;
+      if (p.most == 128) return go(ln_fwd_kernel<TA, TW, kRms, K, 4, 4, 128>, 4);
+      return p.most == 256 ? go(ln_fwd_kernel<TA, TW, kRms, K, 4, 4, 256>, 4)
+                           : go(ln_fwd_kernel<TA, TW, kRms, K, 4, 3, 768>, 3);
+    };
+    auto typed = [&](auto tw) {
+      if constexpr (!kRms)
+        if (b) return sized(tw, std::integral_constant<int, 2>());
+      return sized(tw, std::integral_constant<int, 1>());
+    };
+    if (!w) return sized(TA(), std::integral_constant<int, 0>());
+    if (f32) return typed(float());
+    return typed(TA());
+  }
+  if (p.per) {
+    auto go = [&](auto kernel) {  // nothing is kept from row to row: a CTA a row
+      kernel<<<row_grid((rows + p.shape.groups - 1) / p.shape.groups), p.shape.threads, 0, st>>>(
+          X, ldx, w, b, f32, eps, Y, mean, rstd, rows, int(cols), p.shape.tpr, p.shape.groups);
+      return check_launch();
+    };
+    if (p.most == 128) return go(ln_fwd_element_kernel<TA, kRms, 4, 128>);
+    return p.per == 4 ? go(ln_fwd_element_kernel<TA, kRms, 4, 512>) : go(ln_fwd_element_kernel<TA, kRms, 16, 512>);
+  }
+  ln_fwd_wide_kernel<TA, kRms><<<row_grid(rows), kT, 0, st>>>(X, ldx, w, b, f32, eps, Y, mean, rstd, rows, cols);
+  return check_launch();
+}
+
+// Slabs of rows that the column kernel for wide rows works on.
+int slabs_wide(int64_t rows, int64_t cols) {
   const int64_t tiles = (cols + kT - 1) / kT;
   int64_t z = (int64_t(num_sms()) * 8 + tiles - 1) / tiles;
   if (z > rows) z = rows;
   return int(z < 1 ? 1 : z > 1024 ? 1024 : z);
 }
 
-template <typename TA, typename TW, bool kRms>
-int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, float eps, void* y, float* mean, float* rstd,
-               int64_t rows, int64_t cols, cudaStream_t st) {
-  ln_fwd_any_kernel<TA, TW, kRms><<<row_grid(rows), kT, 0, st>>>(
-      static_cast<const TA*>(x), ldx, static_cast<const TW*>(w), static_cast<const TW*>(b), eps, static_cast<TA*>(y),
-      mean, rstd, rows, cols);
-  return check_launch();
-}
-
-template <typename TA, typename TW, bool kRms>
-int launch_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
-               const float* rstd, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, int64_t rows, int64_t cols,
-               cudaStream_t st) {
+template <typename TA, bool kRms, bool kCols>
+int launch_bwd_rows(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, bool f32,
+                    const float* mean, const float* rstd, void* dx, float* part, int64_t rows, int64_t cols, int* Z,
+                    cudaStream_t st) {
+  constexpr int V = Vec16<TA>::N;
+  const bool vec = cols % V == 0 && ldx % V == 0 && lddy % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) &&
+                   aligned16(w);
+  const Plan p = plan_rows(rows, vec ? cols / V : cols, vec, false);
   auto D = static_cast<const TA*>(dy);
   auto X = static_cast<const TA*>(x);
-  const int Z = col_slabs(rows, cols);
-  if ((dw || db) && (!ws || ws_bytes < size_t(Z) * 2 * size_t(cols) * 4 || (reinterpret_cast<uintptr_t>(ws) & 15u)))
-    return DORA_ERR_WORKSPACE;
+  auto DX = static_cast<TA*>(dx);
+  *Z = int(p.ctas);
+  if (p.per == 2) {
+    const int S = p.most < 1024 ? 4 : 3;  // 1024 threads' rows fit shared memory three times
+    size_t smem = size_t(S) * 4 * p.shape.threads * 16;
+    if (smem < size_t(cols) * 8 && p.shape.groups > 1) smem = size_t(cols) * 8;
+    auto go = [&](auto kernel) {
+      const int e = allow_shared(kernel, smem);
+      if (e) return e;
+      kernel<<<unsigned(p.ctas), p.shape.threads, smem, st>>>(D, lddy, X, ldx, w, f32, mean, rstd, DX, part, rows,
+                                                              int(cols), p.shape.tpr, p.shape.groups, 1.0f);
+      return check_launch();
+    };
+    if (p.most == 128) return go(ln_bwd_kernel<TA, kRms, 2, 4, 128, kCols>);
+    return p.most == 512 ? go(ln_bwd_kernel<TA, kRms, 2, 4, 512, kCols>) : go(ln_bwd_kernel<TA, kRms, 2, 3, 1024, kCols>);
+  }
+  if (p.per) {
+    const size_t smem = kCols && p.shape.groups > 1 ? size_t(cols) * 8 : 0;
+    auto go = [&](auto kernel) {
+      kernel<<<unsigned(p.ctas), p.shape.threads, smem, st>>>(D, lddy, X, ldx, w, f32, mean, rstd, DX, part, rows,
+                                                              int(cols), p.shape.tpr, p.shape.groups);
+      return check_launch();
+    };
+    if (p.most == 128) return go(ln_bwd_element_kernel<TA, kRms, 4, 128, kCols>);
+    return p.per == 4 ? go(ln_bwd_element_kernel<TA, kRms, 4, 512, kCols>)
+                      : go(ln_bwd_element_kernel<TA, kRms, 16, 512, kCols>);
+  }
   if (dx && rows) {
-    ln_bwd_any_kernel<TA, TW, kRms><<<row_grid(rows), kT, 0, st>>>(D, lddy, X, ldx, static_cast<const TW*>(w), mean,
-                                                                   rstd, static_cast<TA*>(dx), rows, cols);
+    ln_bwd_wide_kernel<TA, kRms><<<row_grid(rows), kT, 0, st>>>(D, lddy, X, ldx, w, f32, mean, rstd, DX, rows, cols);
     const int e = check_launch();
     if (e) return e;
   }
-  if (!dw && !db) return DORA_OK;
-  const unsigned tiles = unsigned((cols + kT - 1) / kT);
+  if (!kCols) return DORA_OK;
+  *Z = slabs_wide(rows, cols);
+  ln_col_wide_kernel<TA, kRms><<<dim3(unsigned((cols + kT - 1) / kT), unsigned(*Z)), kT, 0, st>>>(
+      D, lddy, X, ldx, mean, rstd, part, rows, cols);
+  return check_launch();
+}
+
+size_t bwd_workspace(int64_t rows, int64_t cols) {  // of any type and alignment
+  int64_t z = 1;
+  for (int V : {1, 4, 8}) {
+    const Plan p = plan_rows(rows, (cols + V - 1) / V, V > 1, false);
+    const int64_t n = p.per ? p.ctas : slabs_wide(rows, cols);
+    if (n > z) z = n;
+  }
+  return size_t(z) * 2 * size_t(cols) * 4;
+}
+
+template <typename TA, bool kRms>
+int launch_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, bool f32, const float* mean,
+               const float* rstd, void* dx, void* dw, void* db, void* ws, size_t ws_bytes, int64_t rows, int64_t cols,
+               cudaStream_t st) {
+  const bool sums = dw || db;
+  if (sums && (!ws || ws_bytes < bwd_workspace(rows, cols) || !aligned16(ws))) return DORA_ERR_WORKSPACE;
   auto part = static_cast<float*>(ws);
-  ln_col_any_kernel<TA, kRms><<<dim3(tiles, unsigned(Z)), kT, 0, st>>>(D, lddy, X, ldx, mean, rstd, part, rows, cols);
-  const int e = check_launch();
-  if (e) return e;
-  ln_col_finish_kernel<TW><<<tiles, kT, 0, st>>>(part, Z, static_cast<TW*>(dw), static_cast<TW*>(db), cols);
+  int Z = 0;
+  const int e = sums ? launch_bwd_rows<TA, kRms, true>(dy, lddy, x, ldx, w, f32, mean, rstd, dx, part, rows, cols, &Z, st)
+                     : launch_bwd_rows<TA, kRms, false>(dy, lddy, x, ldx, w, f32, mean, rstd, dx, part, rows, cols, &Z, st);
+  if (e || !sums) return e;
+  const dim3 grid(unsigned((cols + 31) / 32), db ? 2 : 1);
+  if (f32) ln_col_finish_kernel<float><<<grid, kT, 0, st>>>(part, Z, static_cast<float*>(dw), static_cast<float*>(db), int(cols));
+  else ln_col_finish_kernel<TA><<<grid, kT, 0, st>>>(part, Z, static_cast<TA*>(dw), static_cast<TA*>(db), int(cols));
   return check_launch();
 }
 
@@ -172,13 +799,12 @@ bool types_ok(int act_dtype, int w_dtype) {
   return dtype_ok(act_dtype) && (w_dtype == act_dtype || w_dtype == DORA_DTYPE_F32);
 }
 
-template <bool kRms, typename F>
-int by_type(int act_dtype, int w_dtype, F f) {
+template <typename F>
+int by_type(int act_dtype, F f) {
   switch (act_dtype) {
-    case DORA_DTYPE_BF16:
-      return w_dtype == DORA_DTYPE_F32 ? f(__nv_bfloat16(), float()) : f(__nv_bfloat16(), __nv_bfloat16());
-    case DORA_DTYPE_F16: return w_dtype == DORA_DTYPE_F32 ? f(__half(), float()) : f(__half(), __half());
-    default: return f(float(), float());
+    case DORA_DTYPE_BF16: return f(__nv_bfloat16());
+    case DORA_DTYPE_F16: return f(__half());
+    default: return f(float());
   }
 }
 
@@ -188,10 +814,10 @@ int norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int w_dty
   if (!shape_ok(rows, cols, ldx) || !types_ok(act_dtype, w_dtype) || !(eps >= 0)) return DORA_ERR_INVALID_ARGUMENT;
   if (rows == 0 || cols == 0) return DORA_OK;
   if (!x || !y || x == y) return DORA_ERR_INVALID_ARGUMENT;
-  return by_type<kRms>(act_dtype, w_dtype, [&](auto ta, auto tw) {
-    return launch_fwd<decltype(ta), decltype(tw), kRms>(x, ldx, w, b, float(eps), y, static_cast<float*>(mean),
-                                                        static_cast<float*>(rstd), rows, cols,
-                                                        static_cast<cudaStream_t>(stream));
+  return by_type(act_dtype, [&](auto t) {
+    return launch_fwd<decltype(t), kRms>(x, ldx, w, b, w_dtype == DORA_DTYPE_F32, float(eps), y,
+                                         static_cast<float*>(mean), static_cast<float*>(rstd), rows, cols,
+                                         static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -203,10 +829,10 @@ int norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const voi
   if (cols == 0 || (!dx && !dw && !db)) return DORA_OK;
   if (rows && (!dy || !x || !rstd || (!kRms && !mean) || (dx && (dx == dy || dx == x)))) return DORA_ERR_INVALID_ARGUMENT;
   if (rows == 0 && !dw && !db) return DORA_OK;
-  return by_type<kRms>(act_dtype, w_dtype, [&](auto ta, auto tw) {
-    return launch_bwd<decltype(ta), decltype(tw), kRms>(dy, lddy, x, ldx, w, static_cast<const float*>(mean),
-                                                        static_cast<const float*>(rstd), dx, dw, db, ws, ws_bytes, rows,
-                                                        cols, static_cast<cudaStream_t>(stream));
+  return by_type(act_dtype, [&](auto t) {
+    return launch_bwd<decltype(t), kRms>(dy, lddy, x, ldx, w, w_dtype == DORA_DTYPE_F32,
+                                         static_cast<const float*>(mean), static_cast<const float*>(rstd), dx, dw, db,
+                                         ws, ws_bytes, rows, cols, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -228,7 +854,7 @@ extern "C" int dora_rms_norm_fwd(const void* x, int64_t ldx, const void* weight,
 
 extern "C" size_t dora_layer_norm_bwd_workspace_size(int64_t rows, int64_t cols) {
   if (!shape_ok(rows, cols, cols) || cols == 0) return 0;
-  return size_t(col_slabs(rows, cols)) * 2 * size_t(cols) * 4;
+  return bwd_workspace(rows, cols);
 }
 
 extern "C" int dora_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight,
