@@ -392,30 +392,118 @@ ln_bwd_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x,
 }
 
 // ---------------------------------------------------------------------------
-// Rows that start or end off a 16-byte boundary: the same by elements, read
-// straight from global memory (the backward's second time from L2).
+// Rows that start or end off a 16-byte boundary.  They come and go in 16-byte pieces all the
+// same, cut at multiples of 16 in memory, and stand in shared memory as they stand there;
+// a thread takes every tpr-th element.  (Loads and stores of single elements took 7 times as
+// long at 16384 x 5003 in bf16.)
 // ---------------------------------------------------------------------------
+__host__ __device__ constexpr int row_pieces(int cols, int size) { return (cols * size + 30) / 16; }
+
+template <bool kWide> __device__ __forceinline__ void row_sync() {
+  if constexpr (kWide) __syncthreads();
+  else __syncwarp();
+}
+
+// Copies `cols` elements at `from` to shared memory, piece by piece, the way they stand in memory.  The first piece
+// may start in the row before (of the same buffer, from `base` on); where that would be outside, and at the
+// row's end, only what belongs to the row is read.
+template <typename T>
+__device__ __forceinline__ void fetch_pieces(uint4* to, const T* from, const T* base, int cols, int t, int tpr) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(from), end = a + cols * sizeof(T);
+  const uintptr_t a0 = a & ~uintptr_t(15);
+  const uint32_t dst = shared_addr(to);
+  for (int u = t; a0 + u * 16 < end; u += tpr) {
+    const uintptr_t src = a0 + u * 16;
+    if (src < reinterpret_cast<uintptr_t>(base)) {
+      T* e = reinterpret_cast<T*>(to + u);
+      for (int i = 0; i < int(16 / sizeof(T)); ++i) {
+        const uintptr_t q = src + i * sizeof(T);
+        if (q >= a && q < end) e[i] = *reinterpret_cast<const T*>(q);
+      }
+    } else {
+      const int bytes = end - src < 16 ? int(end - src) : 16;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + u * 16), "l"(src), "r"(bytes) : "memory");
+    }
+  }
+}
+// The other way: `cols` elements that stand in shared memory the way they are to stand at `to`.
+template <typename T>
+__device__ __forceinline__ void store_pieces(T* to, const uint4* from, int cols, int t, int tpr) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(to), end = a + cols * sizeof(T);
+  const uintptr_t a0 = a & ~uintptr_t(15);
+  for (int u = t; a0 + u * 16 < end; u += tpr) {
+    const uintptr_t dst = a0 + u * 16;
+    if (dst >= a && dst + 16 <= end) {
+      st_stream(reinterpret_cast<void*>(dst), from[u]);
+    } else {
+      const T* e = reinterpret_cast<const T*>(from + u);
+      for (int i = 0; i < int(16 / sizeof(T)); ++i) {
+        const uintptr_t q = dst + i * sizeof(T);
+        if (q >= a && q < end) *reinterpret_cast<T*>(q) = e[i];
+      }
+    }
+  }
+}
+// Where element 0 of the row at p stands in its first piece.
+template <typename T> __device__ __forceinline__ int in_piece(const T* p) {
+  return int(reinterpret_cast<uintptr_t>(p) & 15) / int(sizeof(T));
+}
+// f = f * w, or f + w, for this thread's elements of a row.
+template <typename TA, int PER, bool kAdd>
+__device__ __forceinline__ void with_param(const void* w, bool f32, int t, int tpr, int cols, float (&f)[PER]) {
+  if (!w) return;
+  float v[PER];
+  if (f32) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) v[p] = p * tpr + t < cols ? __ldg(static_cast<const float*>(w) + p * tpr + t) : 0.f;
+  } else {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) v[p] = p * tpr + t < cols ? to_f32(static_cast<const TA*>(w)[p * tpr + t]) : 0.f;
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p) f[p] = kAdd ? f[p] + v[p] : __fmul_rn(f[p], v[p]);
+}
+
+constexpr int kPieceStages = 3;
+constexpr int kPieceFill = 768;  // threads of these kernels an SM holds (1024 of those for the widest rows)
+
 template <typename TA, bool kRms, int PER, int kMax>
-__global__ void __launch_bounds__(kMax)
-ln_fwd_element_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b,
-                      bool f32, float eps, TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
-                      int64_t rows, int cols, int tpr, int groups) {
+__global__ void __launch_bounds__(kMax, kPieceFill / kMax)
+ln_fwd_pieces_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b,
+                     bool f32, float eps, TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd,
+                     int64_t rows, int cols, int tpr, int groups) {
+  constexpr bool kWide = kMax > 128;
+  constexpr int S = kPieceStages;
+  extern __shared__ uint4 ring[];  // [groups][S + 1][pieces]: S rows coming, one going
   DORA_ROW_SUM(sum, kMax, 1);
   const Walk at = walk(rows, tpr, groups);
+  const int pieces = row_pieces(cols, sizeof(TA));
+  uint4* mine = ring + at.group * (S + 1) * pieces;
+  uint4* out = mine + S * pieces;
   const float inv = 1.0f / float(cols);
+  const TA* from = x + at.first * ldx;
+  auto fetch = [&](int64_t k, int s) {
+    if (k < at.mine) fetch_pieces(mine + s * pieces, from + k * at.step * ldx, x, cols, at.t, tpr);
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s, s);
+  int s = 0;
   for (int64_t k = 0; k < at.rounds; ++k) {
-    const bool live = k < at.mine;
+    copies_done<S - 2>();
+    row_sync<kWide>();  // the row is there, and everybody is done with the one before
+    fetch(k + S - 1, s == 0 ? S - 1 : s - 1);
+    const bool live = kWide || k < at.mine;
     const int64_t r = at.first + k * at.step;
-    const TA* xr = x + r * ldx;
-    float f[PER];
-    float a = 0.f;
+    const TA* row = reinterpret_cast<const TA*>(mine + s * pieces) + in_piece(x + r * ldx);
+    s = s == S - 1 ? 0 : s + 1;
+    float f[PER], one[1] = {0.f};
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int c = p * tpr + at.t;
-      f[p] = live && c < cols ? to_f32(xr[c]) : 0.f;
-      a += f[p];
+      f[p] = live && c < cols ? to_f32(row[c]) : 0.f;
+      one[0] += f[p];
     }
-    float one[1] = {a};
     if constexpr (!kRms) sum(one);
     const float mu = kRms ? 0.f : one[0] * inv;
     one[0] = 0.f;
@@ -427,68 +515,101 @@ ln_fwd_element_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restr
       }
     sum(one);
     const float rs = rsqrtf(one[0] * inv + eps);
-    if (!live) continue;
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int c = p * tpr + at.t;
-      if (c < cols) y[r * cols + c] = from_f32<TA>(fmaf(f[p] * rs, param<TA>(w, f32, c, 1.f), param<TA>(b, f32, c, 0.f)));
-    }
-    if (at.t == 0) {
-      if (!kRms && mean) mean[r] = mu;
-      if (rstd) rstd[r] = rs;
+    for (int p = 0; p < PER; ++p) f[p] *= rs;
+    with_param<TA, PER, false>(w, f32, at.t, tpr, cols, f);
+    with_param<TA, PER, true>(b, f32, at.t, tpr, cols, f);
+    TA* to = reinterpret_cast<TA*>(out) + in_piece(y + r * cols);
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (live && p * tpr + at.t < cols) to[p * tpr + at.t] = from_f32<TA>(f[p]);
+    row_sync<kWide>();
+    if (live) {
+      store_pieces(y + r * cols, out, cols, at.t, tpr);
+      if (at.t == 0) {
+        if (!kRms && mean) mean[r] = mu;
+        if (rstd) rstd[r] = rs;
+      }
     }
   }
 }
 
 template <typename TA, bool kRms, int PER, int kMax, bool kCols>
-__global__ void __launch_bounds__(kMax)
-ln_bwd_element_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
-                      const void* __restrict__ w, bool f32, const float* __restrict__ mean,
-                      const float* __restrict__ rstd, TA* __restrict__ dx, float* __restrict__ partial, int64_t rows,
-                      int cols, int tpr, int groups) {
-  extern __shared__ float joined[];  // [2][cols] where a CTA works on several rows
+__global__ void __launch_bounds__(kMax, kPieceFill / kMax)
+ln_bwd_pieces_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict__ x, int64_t ldx,
+                     const void* __restrict__ w, bool f32, const float* __restrict__ mean,
+                     const float* __restrict__ rstd, TA* __restrict__ dx, float* __restrict__ partial, int64_t rows,
+                     int cols, int tpr, int groups) {
+  constexpr bool kWide = kMax > 128;
+  constexpr int S = kPieceStages;
+  extern __shared__ uint4 ring[];  // [groups][2 S + 1][pieces]: S rows of dy and x coming, one of dx going
   DORA_ROW_SUM(sum, kMax, 2);
   const Walk at = walk(rows, tpr, groups);
+  const int pieces = row_pieces(cols, sizeof(TA));
+  uint4* mine = ring + at.group * (2 * S + 1) * pieces;
+  uint4* out = mine + 2 * S * pieces;
   const float inv = 1.0f / float(cols);
   float dw[kCols ? PER : 1] = {}, db[kCols && !kRms ? PER : 1] = {};
+  auto fetch = [&](int64_t k, int s) {
+    if (k < at.mine) {
+      const int64_t r = at.first + k * at.step;
+      fetch_pieces(mine + 2 * s * pieces, dy + r * lddy, dy, cols, at.t, tpr);
+      fetch_pieces(mine + (2 * s + 1) * pieces, x + r * ldx, x, cols, at.t, tpr);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s, s);
+  int s = 0;
   for (int64_t k = 0; k < at.rounds; ++k) {
-    const bool live = k < at.mine;
+    const bool live = kWide || k < at.mine;
     const int64_t r = at.first + k * at.step;
-    const TA *xr = x + r * ldx, *dr = dy + r * lddy;
     float mu = 0.f, rs = 0.f;
     if (live) {
       if constexpr (!kRms) mu = mean[r];
       rs = rstd[r];
     }
-    float s0 = 0.f, s1 = 0.f;
+    copies_done<S - 2>();
+    row_sync<kWide>();  // the row is there, and everybody is done with the one before
+    fetch(k + S - 1, s == 0 ? S - 1 : s - 1);
+    const TA* dr = reinterpret_cast<const TA*>(mine + 2 * s * pieces) + in_piece(dy + r * lddy);
+    const TA* xr = reinterpret_cast<const TA*>(mine + (2 * s + 1) * pieces) + in_piece(x + r * ldx);
+    s = s == S - 1 ? 0 : s + 1;
+    float a[PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) a[p] = live && p * tpr + at.t < cols ? to_f32(dr[p * tpr + at.t]) : 0.f;
+    with_param<TA, PER, false>(w, f32, at.t, tpr, cols, a);
+    float c01[2] = {0.f, 0.f};
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int c = p * tpr + at.t;
       if (live && c < cols) {
-        const float d = to_f32(dr[c]), h = (to_f32(xr[c]) - mu) * rs, a = __fmul_rn(d, param<TA>(w, f32, c, 1.f));
-        s0 += a;
-        s1 = fmaf(a, h, s1);
-        if constexpr (kCols) dw[p] = fmaf(d, h, dw[p]);
-        if constexpr (kCols && !kRms) db[p] += d;
-      }
-    }
-    if (dx) {  // the same for all threads
-      float c01[2] = {s0, s1};
-      sum(c01);
-      const float c0 = kRms ? 0.f : c01[0] * inv, c1 = c01[1] * inv;
-#pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        const int c = p * tpr + at.t;
-        if (live && c < cols) {
-          const float a = __fmul_rn(to_f32(dr[c]), param<TA>(w, f32, c, 1.f));
-          dx[r * cols + c] = from_f32<TA>((a - c0 - (to_f32(xr[c]) - mu) * rs * c1) * rs);
+        const float h = (to_f32(xr[c]) - mu) * rs;
+        c01[0] += a[p];
+        c01[1] = fmaf(a[p], h, c01[1]);
+        if constexpr (kCols) {
+          const float d = to_f32(dr[c]);
+          dw[p] = fmaf(d, h, dw[p]);
+          if constexpr (!kRms) db[p] += d;
         }
       }
     }
+    if (!dx) continue;  // the same for all threads
+    sum(c01);
+    const float c0 = kRms ? 0.f : c01[0] * inv, c1 = c01[1] * inv;
+    TA* to = reinterpret_cast<TA*>(out) + in_piece(dx + r * cols);
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int c = p * tpr + at.t;
+      if (live && c < cols) to[c] = from_f32<TA>((a[p] - c0 - (to_f32(xr[c]) - mu) * rs * c1) * rs);
+    }
+    row_sync<kWide>();
+    if (live) store_pieces(dx + r * cols, out, cols, at.t, tpr);
   }
   if constexpr (kCols) {
-    float* out = partial + int64_t(blockIdx.x) * 2 * cols;
-    float* acc = groups > 1 ? joined : out;
+    copies_done<0>();
+    float* to = partial + int64_t(blockIdx.x) * 2 * cols;
+    float* acc = groups > 1 ? reinterpret_cast<float*>(ring) : to;  // the groups add up in shared memory, one by one
     for (int g = 0; g < groups; ++g) {
       if (groups > 1) __syncthreads();
       if (at.group == g)
@@ -503,7 +624,7 @@ ln_bwd_element_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restr
     }
     if (groups > 1) {
       __syncthreads();
-      for (int c = threadIdx.x; c < (kRms ? 1 : 2) * cols; c += blockDim.x) out[c] = acc[c];
+      for (int c = threadIdx.x; c < (kRms ? 1 : 2) * cols; c += blockDim.x) to[c] = acc[c];
     }
   }
 }
@@ -633,26 +754,45 @@ ln_col_wide_kernel(const TA* __restrict__ dy, int64_t lddy, const TA* __restrict
 // ---------------------------------------------------------------------------
 unsigned row_grid(int64_t rows) { return unsigned(rows < (1 << 20) ? rows : (1 << 20)); }
 
-// How the threads of the row kernels share rows of `units` (16-byte vectors, or elements).
+// How the threads of the row kernels share rows.
 struct Plan {
-  int per, most;  // units a thread holds, threads a CTA has at most; per 0: rows too wide
-  Shape shape;
-  int64_t ctas;
+  int per = 0, most = 0;  // units (elements) a thread holds, threads a CTA has at most; per 0: not for these rows
+  Shape shape = {};
+  int64_t ctas = 0;
+  size_t shared = 0;
 };
-// `fill`: threads that an SM's registers hold, 64 of them a thread in the forward and 128 in the backward.  More
-// CTAs than fill the GPU would only divide the walk down the rows, and multiply the partial sums.
-Plan plan_rows(int64_t rows, int64_t units, bool vec, bool fwd) {
+// CTAs that walk down the rows: as many as the SMs hold, but in the backward, whose every CTA leaves a row of partial
+// sums to be read again, at least eight rows to one as long as every SM has one.
+int64_t walkers(const Shape& s, int64_t rows, int per_sm, bool fwd) {
+  const int64_t need = (rows + s.groups - 1) / s.groups, held = int64_t(num_sms()) * (per_sm > 1 ? per_sm : 1);
+  int64_t n = need < held ? need : held;
+  if (!fwd && n > num_sms() && n > need / 8) n = need / 8 > num_sms() ? need / 8 : num_sms();
+  return n < 1 ? 1 : n;
+}
+// 16-byte units: 80 registers a thread in the forward (768 threads an SM), 128 in the backward (512; 64 for rows
+// of more than 1024 units).
+Plan plan_units(int64_t rows, int64_t units, bool fwd) {
   Plan p;
-  const int fill = fwd ? kFwdFill : kBwdFill;
-  if (vec && fwd) p.per = units <= 768 * 4 ? 4 : 0;
-  else p.per = vec ? (units <= 2048 ? 2 : 0) : units <= 2048 ? 4 : units <= 8192 ? 16 : 0;
+  p.per = fwd ? (units <= 768 * 4 ? 4 : 0) : units <= 2048 ? 2 : 0;
   if (!p.per) return p;
   p.shape = share_row(units, p.per, 128);
-  if (vec && fwd) p.most = p.shape.groups > 1 ? 128 : p.shape.threads > 256 ? 768 : 256;
-  else p.most = p.shape.groups > 1 ? 128 : vec && units > 1024 ? 1024 : 512;
-  const int64_t held = int64_t(num_sms()) * (fill > p.shape.threads ? fill / p.shape.threads : 1);
-  const int64_t need = (rows + p.shape.groups - 1) / p.shape.groups;
-  p.ctas = need < 1 ? 1 : need < held ? need : held;
+  if (fwd) p.most = p.shape.groups > 1 ? 128 : p.shape.threads > 256 ? 768 : 256;
+  else p.most = p.shape.groups > 1 ? 128 : units > 1024 ? 1024 : 512;
+  p.ctas = walkers(p.shape, rows, (fwd ? kFwdFill : kBwdFill) / p.shape.threads, fwd);
+  return p;
+}
+// Elements, with `buffers` rows in shared memory (200 KB of it an SM).
+Plan plan_pieces(int64_t rows, int64_t cols, int size, int buffers) {
+  Plan p;
+  if (cols > 16384) return p;
+  p.per = cols <= 2048 ? 8 : 16;
+  p.shape = share_row(cols, p.per, 128);
+  p.most = p.shape.groups > 1 ? 128 : cols <= 2048 ? 256 : cols <= 6144 ? 384 : 1024;
+  p.shared = size_t(p.shape.groups) * buffers * row_pieces(int(cols), size) * 16;
+  if (p.shared > 220 * 1024) return Plan();
+  const int fill = p.most == 1024 ? 1024 : kPieceFill;
+  const int by_threads = fill / p.shape.threads, by_shared = int(200 * 1024 / (p.shared + 1024));
+  p.ctas = walkers(p.shape, rows, by_threads < by_shared ? by_threads : by_shared, buffers <= kPieceStages + 1);
   return p;
 }
 
@@ -667,7 +807,7 @@ int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, bool f3
                float* rstd, int64_t rows, int64_t cols, cudaStream_t st) {
   constexpr int V = Vec16<TA>::N;
   const bool vec = cols % V == 0 && ldx % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
-  const Plan p = plan_rows(rows, vec ? cols / V : cols, vec, true);
+  const Plan p = vec ? plan_units(rows, cols / V, true) : Plan();
   auto X = static_cast<const TA*>(x);
   auto Y = static_cast<TA*>(y);
   if (p.per && vec && (w || !b)) {
@@ -695,14 +835,18 @@ int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, bool f3
     if (f32) return typed(float());
     return typed(TA());
   }
-  if (p.per) {
-    auto go = [&](auto kernel) {  // nothing is kept from row to row: a CTA a row
-      kernel<<<row_grid((rows + p.shape.groups - 1) / p.shape.groups), p.shape.threads, 0, st>>>(
-          X, ldx, w, b, f32, eps, Y, mean, rstd, rows, int(cols), p.shape.tpr, p.shape.groups);
+  const Plan q = plan_pieces(rows, cols, int(sizeof(TA)), kPieceStages + 1);
+  if (q.per) {
+    auto go = [&](auto kernel) {
+      const int e = allow_shared(kernel, q.shared);
+      if (e) return e;
+      kernel<<<unsigned(q.ctas), q.shape.threads, q.shared, st>>>(X, ldx, w, b, f32, eps, Y, mean, rstd, rows, int(cols),
+                                                                  q.shape.tpr, q.shape.groups);
       return check_launch();
     };
-    if (p.most == 128) return go(ln_fwd_element_kernel<TA, kRms, 4, 128>);
-    return p.per == 4 ? go(ln_fwd_element_kernel<TA, kRms, 4, 512>) : go(ln_fwd_element_kernel<TA, kRms, 16, 512>);
+    if (q.most == 128) return go(ln_fwd_pieces_kernel<TA, kRms, 8, 128>);
+    if (q.most == 256) return go(ln_fwd_pieces_kernel<TA, kRms, 8, 256>);
+    return q.most == 384 ? go(ln_fwd_pieces_kernel<TA, kRms, 16, 384>) : go(ln_fwd_pieces_kernel<TA, kRms, 16, 1024>);
   }
   ln_fwd_wide_kernel<TA, kRms><<<row_grid(rows), kT, 0, st>>>(X, ldx, w, b, f32, eps, Y, mean, rstd, rows, cols);
   return check_launch();
@@ -723,12 +867,12 @@ int launch_bwd_rows(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
   constexpr int V = Vec16<TA>::N;
   const bool vec = cols % V == 0 && ldx % V == 0 && lddy % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) &&
                    aligned16(w);
-  const Plan p = plan_rows(rows, vec ? cols / V : cols, vec, false);
+  const Plan p = vec ? plan_units(rows, cols / V, false) : Plan();
   auto D = static_cast<const TA*>(dy);
   auto X = static_cast<const TA*>(x);
   auto DX = static_cast<TA*>(dx);
   *Z = int(p.ctas);
-  if (p.per == 2) {
+  if (p.per) {
     const int S = p.most < 1024 ? 4 : 3;  // 1024 threads' rows fit shared memory three times
     size_t smem = size_t(S) * 4 * p.shape.threads * 16;
     if (smem < size_t(cols) * 8 && p.shape.groups > 1) smem = size_t(cols) * 8;
@@ -742,16 +886,21 @@ int launch_bwd_rows(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
     if (p.most == 128) return go(ln_bwd_kernel<TA, kRms, 2, 4, 128, kCols>);
     return p.most == 512 ? go(ln_bwd_kernel<TA, kRms, 2, 4, 512, kCols>) : go(ln_bwd_kernel<TA, kRms, 2, 3, 1024, kCols>);
   }
-  if (p.per) {
-    const size_t smem = kCols && p.shape.groups > 1 ? size_t(cols) * 8 : 0;
+  const Plan q = plan_pieces(rows, cols, int(sizeof(TA)), 2 * kPieceStages + 1);
+  if (q.per) {
+    const size_t smem = kCols && q.shape.groups > 1 && q.shared < size_t(cols) * 8 ? size_t(cols) * 8 : q.shared;
+    *Z = int(q.ctas);
     auto go = [&](auto kernel) {
-      kernel<<<unsigned(p.ctas), p.shape.threads, smem, st>>>(D, lddy, X, ldx, w, f32, mean, rstd, DX, part, rows,
-                                                              int(cols), p.shape.tpr, p.shape.groups);
+      const int e = allow_shared(kernel, smem);
+      if (e) return e;
+      kernel<<<unsigned(q.ctas), q.shape.threads, smem, st>>>(D, lddy, X, ldx, w, f32, mean, rstd, DX, part, rows,
+                                                              int(cols), q.shape.tpr, q.shape.groups);
       return check_launch();
     };
-    if (p.most == 128) return go(ln_bwd_element_kernel<TA, kRms, 4, 128, kCols>);
-    return p.per == 4 ? go(ln_bwd_element_kernel<TA, kRms, 4, 512, kCols>)
-                      : go(ln_bwd_element_kernel<TA, kRms, 16, 512, kCols>);
+    if (q.most == 128) return go(ln_bwd_pieces_kernel<TA, kRms, 8, 128, kCols>);
+    if (q.most == 256) return go(ln_bwd_pieces_kernel<TA, kRms, 8, 256, kCols>);
+    return q.most == 384 ? go(ln_bwd_pieces_kernel<TA, kRms, 16, 384, kCols>)
+                         : go(ln_bwd_pieces_kernel<TA, kRms, 16, 1024, kCols>);
   }
   if (dx && rows) {
     ln_bwd_wide_kernel<TA, kRms><<<row_grid(rows), kT, 0, st>>>(D, lddy, X, ldx, w, f32, mean, rstd, DX, rows, cols);
@@ -767,10 +916,11 @@ int launch_bwd_rows(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
 
 size_t bwd_workspace(int64_t rows, int64_t cols) {  // of any type and alignment
   int64_t z = 1;
-  for (int V : {1, 4, 8}) {
-    const Plan p = plan_rows(rows, (cols + V - 1) / V, V > 1, false);
-    const int64_t n = p.per ? p.ctas : slabs_wide(rows, cols);
-    if (n > z) z = n;
+  for (int V : {4, 8}) {
+    const Plan p = plan_units(rows, (cols + V - 1) / V, false);
+    const Plan q = plan_pieces(rows, cols, 16 / V, 2 * kPieceStages + 1);
+    for (const int64_t n : {p.ctas, q.ctas, int64_t(p.per && q.per ? 0 : slabs_wide(rows, cols))})
+      if (n > z) z = n;
   }
   return size_t(z) * 2 * size_t(cols) * 4;
 }
