@@ -15,9 +15,12 @@
 // error word.  A row of -inf alone has L = -inf, log probabilities -inf, entropy 0 and
 // gradient 0; a row with a NaN or +inf has no distribution: its values are NaN and its
 // alternatives are columns 0 .. k-1.
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
-#include "dora_common.cuh"
+#include <type_traits>
+
+#include "pair.cuh"
 
 namespace dora {
 namespace {
@@ -50,6 +53,8 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
 }
 __device__ __forceinline__ uint32_t key_col(unsigned long long k) { return 0xffffffffu - uint32_t(k); }
 
+__device__ __forceinline__ uint32_t order_bits(float v) { return uint32_t(order_key(v, 0) >> 32); }
+
 template <typename V, typename Op>
 __device__ __forceinline__ V block_fold(V v, V* red, Op op) {
 #pragma unroll
@@ -61,7 +66,6 @@ __device__ __forceinline__ V block_fold(V v, V* red, Op op) {
   __syncthreads();
   return t;
 }
-
 struct Sum {
   template <typename V> __device__ V operator()(V a, V b) const { return a + b; }
 };
@@ -70,110 +74,414 @@ struct Max {
   __device__ unsigned long long operator()(unsigned long long a, unsigned long long b) const { return a > b ? a : b; }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kT)
-logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ targets, int64_t ignore,
-                    float s, float inv_temp, float* __restrict__ logprobs, float* __restrict__ lse,
-                    float* __restrict__ entropy, int k, float* __restrict__ top_lp, int64_t* __restrict__ top_idx,
-                    int64_t rows, int64_t vocab) {
-  __shared__ float red[kT / 32];
-  __shared__ double redd[kT / 32];
-  __shared__ unsigned long long redk[kT / 32];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t target = targets[r];
-    if (target == ignore) {
-      if (threadIdx.x == 0) {
-        logprobs[r] = 0.f;
-        lse[r] = 0.f;
-        if (entropy) entropy[r] = 0.f;
-      }
-      for (int i = threadIdx.x; i < k; i += kT) {
-        top_lp[r * k + i] = 0.f;
-        top_idx[r * k + i] = -1;
-      }
-      continue;
-    }
-    const T* x = logits + r * ld;
-    float m = -CUDART_INF_F;
-    for (int64_t c = threadIdx.x; c < vocab; c += kT) m = fmaxf(m, to_f32(x[c]));
-    m = block_fold(m, red, Max());
-    const float m0 = m == -CUDART_INF_F ? 0.f : m;
-    float sum = 0.f, dot = 0.f;
-    for (int64_t c = threadIdx.x; c < vocab; c += kT) {
-      const float t = (to_f32(x[c]) - m0) * s;
-      const float e = exp2_approx(t);
-      sum += e;
-      dot = fmaf(e, fmaxf(t, -200.f), dot);
-    }
-    const double total = block_fold(double(sum), redd, Sum());
-    const double dots = block_fold(double(dot), redd, Sum());
-    const bool none = m == -CUDART_INF_F && total == 0.0;  // every logit is -inf
-    const float ln_sum = none ? -CUDART_INF_F : log1pf(float(total - 1.0));
-    if (threadIdx.x == 0) {
-      float lp = CUDART_NAN_F;
-      if (target >= 0 && target < vocab) lp = none ? -CUDART_INF_F : fmaf(to_f32(x[target]) - m0, inv_temp, -ln_sum);
-      else record_device_error(DORA_ERR_INVALID_ARGUMENT);
-      logprobs[r] = lp;
-      lse[r] = none ? -CUDART_INF_F : fmaf(m0, inv_temp, ln_sum);
-      if (entropy) entropy[r] = none ? 0.f : ln_sum - kLn2 * float(dots / total);
-    }
-    unsigned long long last = ~0ull;
-    const bool bad = !(total < CUDART_INF);
-    for (int i = 0; i < k; ++i) {
-      unsigned long long best = 0;
-      if (!bad)
-        for (int64_t c = threadIdx.x; c < vocab; c += kT) {
-          const unsigned long long q = order_key(to_f32(x[c]), uint32_t(c));
-          if (q < last && q > best) best = q;
-        }
-      best = block_fold(best, redk, Max());
-      last = best;
-      if (threadIdx.x == 0) {
-        top_lp[r * k + i] = bad ? CUDART_NAN_F : none ? -CUDART_INF_F : fmaf(key_value(best) - m0, inv_temp, -ln_sum);
-        top_idx[r * k + i] = bad ? i : key_col(best);
-      }
-    }
+// A row as 16-byte units at multiples of 16 in memory, and the elements before and after them.
+template <typename T> struct Row {
+  static constexpr int V = Vec16<T>::N;
+  const T* x;
+  int vocab, head, units;
+  __device__ Row(const T* x_, int vocab_) : x(x_), vocab(vocab_) {
+    const int off = int(reinterpret_cast<uintptr_t>(x) & 15) / int(sizeof(T));
+    head = off ? V - off : 0;
+    if (head > vocab) head = vocab;
+    units = (vocab - head) / V;
+  }
+  __device__ int col(int unit) const { return head + unit * V; }
+  // The single column of this thread in the CTA that has the row's first (last) units, -1 if it has none.
+  __device__ int single(bool first, bool last) const {
+    const int t = threadIdx.x;
+    if (first && t < head) return t;
+    const int c = col(units) + t - 32;
+    return last && t >= 32 && c < vocab ? c : -1;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Forward.  A row is one CTA's, or a cluster's whose CTAs take a part each and join over
+// distributed shared memory, so that few rows are read by many SMs.  A thread keeps a
+// maximum and sums relative to it, over 4 units at a time (the next 4 are on their way).
+// Bound by HBM; the exponentials come next (an SM makes 16 a cycle).
+//
+// Alternatives: the k largest elements lie in k groups of elements at most, those with the k
+// largest maxima.  While the row passes, a thread notes the maximum of each of its groups;
+// the k-th largest of the threads' maxima is then a bound that all alternatives reach, and
+// only groups that reach it are read again (about k of them).  Where more than kHeld elements
+// reach it (many equal logits), the k are picked one by one instead.
+// ---------------------------------------------------------------------------
+constexpr int kU = 4;
+constexpr int kGroups = 16;   // groups of a thread's elements
+constexpr int kHeld = 1024;
+
+struct Part {  // of a row, at its maximum
+  float max;
+  double sum, dot;
+};
+
+template <typename T> __device__ __forceinline__ uint4 no_logits() {  // -inf
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
+// Distance of a smaller maximum to a larger one, in powers of two; what is there at 2^-1000 is nothing, and the
+// distance stays finite for -inf and for the types' lowest values.
+__device__ __forceinline__ float below(float m, float to, float s) { return fmaxf((m - to) * s, -1000.f); }
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(a, fmaxf(b, c)); }
+
+// out[r] = the key with r larger ones among the n (all different) in `keys`, for r < k.
+__device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n, int k, unsigned long long* out) {
+  for (int i = threadIdx.x; i < n; i += kT) {
+    const unsigned long long mine = keys[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += keys[j] > mine;
+    if (r < k) out[r] = mine;
   }
 }
 
-template <typename T>
+template <typename T, bool kEntropy, bool kTop>
+__global__ void __launch_bounds__(kT, 3)
+logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ targets, int64_t ignore,
+                    float s, float inv_temp, float* __restrict__ logprobs, float* __restrict__ lse,
+                    float* __restrict__ entropy, int k, float* __restrict__ top_lp, int64_t* __restrict__ top_idx,
+                    int vocab, int ranks) {
+  namespace cg = cooperative_groups;
+  constexpr int V = Vec16<T>::N, N = V / 2;
+  __shared__ float red[kT / 32];
+  __shared__ double redd[kT / 32];
+  __shared__ Part part;
+  __shared__ float group_max[kTop ? kGroups + 1 : 1][kT];  // [kGroups]: the single element
+  __shared__ unsigned long long held[kTop ? kHeld : 1], best[kTop ? kMaxTop : 1], redk[kT / 32];
+  __shared__ uint32_t thread_max[kTop ? kT : 1];
+  __shared__ uint32_t bound;
+  __shared__ int count;
+
+  const int64_t r = blockIdx.x / ranks;
+  const int rank = blockIdx.x % ranks;
+  const int64_t target = targets[r];
+  if (target == ignore) {
+    if (rank == 0) {
+      if (threadIdx.x == 0) {
+        logprobs[r] = 0.f;
+        lse[r] = 0.f;
+        if (kEntropy) entropy[r] = 0.f;
+      }
+      for (int i = threadIdx.x; kTop && i < k; i += kT) {
+        top_lp[r * k + i] = 0.f;
+        top_idx[r * k + i] = -1;
+      }
+    }
+    return;
+  }
+  const Row<T> row(logits + r * ld, vocab);
+  float given = 0.f;
+  if (rank == 0 && threadIdx.x == 0 && target >= 0 && target < vocab) given = to_f32(row.x[target]);
+  const int u0 = int(int64_t(row.units) * rank / ranks), u1 = int(int64_t(row.units) * (rank + 1) / ranks);
+  const int single = row.single(rank == 0, rank == ranks - 1);
+  const uint4* units = reinterpret_cast<const uint4*>(row.x + row.head);
+  const int rounds = (u1 - u0 + kT * kU - 1) / (kT * kU), per_group = (rounds + kGroups - 1) / kGroups;
+
+  float m = -CUDART_INF_F;
+  Two sum = both(0.f), dot = both(0.f);
+  auto raise = [&](float to) {  // the reference of the sums, to a larger maximum
+    if (to > m) {
+      const float by = below(m, to, s), e = exp2_approx(by);
+      if constexpr (kEntropy) dot = mul2(fma2(sum, both(by), dot), both(e));
+      sum = mul2(sum, both(e));
+      m = to;
+    }
+  };
+  auto load = [&](int u, uint4 (&q)[kU]) {
+#pragma unroll
+    for (int j = 0; j < kU; ++j) {
+      const int v = u + j * kT + threadIdx.x;
+      q[j] = v < u1 ? ld_stream(units + v) : no_logits<T>();
+    }
+  };
+  uint4 q[kU];
+  load(u0, q);
+  float group = -CUDART_INF_F;
+  for (int i = 0, u = u0, g = 0; i < rounds; ++i, u += kT * kU) {
+    uint4 next[kU];
+    load(u + kT * kU, next);
+    Two f[kU][N];
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int j = 0; j < kU; ++j) {
+      Pairs<T>::unpack(q[j], f[j]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) top = max3(top, f[j][n].a, f[j][n].b);
+    }
+    raise(top);
+    const Two base = both(m == -CUDART_INF_F ? 0.f : -m);
+#pragma unroll
+    for (int j = 0; j < kU; ++j)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const Two t = mul2(add2(f[j][n], base), both(s));
+        const Two e{exp2_approx(t.a), exp2_approx(t.b)};
+        sum = add2(sum, e);
+        if constexpr (kEntropy) dot = fma2(e, Two{fmaxf(t.a, -200.f), fmaxf(t.b, -200.f)}, dot);
+      }
+    if constexpr (kTop) {
+      group = fmaxf(group, top);
+      if ((i + 1) % per_group == 0 || i + 1 == rounds) {
+        group_max[g++][threadIdx.x] = group;
+        group = -CUDART_INF_F;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kU; ++j) q[j] = next[j];
+  }
+  if (single >= 0) {
+    const float v = to_f32(row.x[single]);
+    raise(v);
+    const float t = (v - (m == -CUDART_INF_F ? 0.f : m)) * s, e = exp2_approx(t);
+    sum.a += e;
+    if constexpr (kEntropy) dot.a = fmaf(e, fmaxf(t, -200.f), dot.a);
+    if constexpr (kTop) group_max[kGroups][threadIdx.x] = v;
+  }
+
+  // Join the threads at the CTA's maximum, in fp64.
+  const float cta_max = block_fold(m, red, Max());
+  {
+    const float by = below(m, cta_max, s), e = exp2_approx(by);
+    const double own = double(sum.a) + double(sum.b);
+    const double total = block_fold(own * e, redd, Sum());
+    double dots = 0.0;
+    if constexpr (kEntropy)
+      dots = block_fold((double(dot.a) + double(dot.b) + by * own) * e, redd, Sum());
+    if (threadIdx.x == 0) part = Part{cta_max, total, dots};
+  }
+
+  if constexpr (kTop) {
+    const bool any = u0 + int(threadIdx.x) < u1 || single >= 0;
+    thread_max[threadIdx.x] = any ? order_bits(m) : 0u;
+    if (threadIdx.x == 0) {
+      bound = 0u;
+      count = 0;
+    }
+    if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0ull;
+    __syncthreads();
+    {
+      const uint32_t mine = thread_max[threadIdx.x];
+      int above = 0;
+      const uint4* all = reinterpret_cast<const uint4*>(thread_max);
+      for (int j = 0; j < kT / 4; ++j) {
+        const uint4 o = all[j];
+        above += (o.x > mine || (o.x == mine && 4 * j < int(threadIdx.x))) +
+                 (o.y > mine || (o.y == mine && 4 * j + 1 < int(threadIdx.x))) +
+                 (o.z > mine || (o.z == mine && 4 * j + 2 < int(threadIdx.x))) +
+                 (o.w > mine || (o.w == mine && 4 * j + 3 < int(threadIdx.x)));
+      }
+      if (above == k - 1) bound = mine;
+    }
+    __syncthreads();
+    const uint32_t least = bound;
+    auto hold = [&](float v, int c) {
+      if (order_bits(v) >= least) {
+        const int at = atomicAdd(&count, 1);  // any order: the keys are ranked
+        if (at < kHeld) held[at] = order_key(v, uint32_t(c));
+      }
+    };
+    if (thread_max[threadIdx.x] >= least) {
+      for (int i = 0; i < rounds; ++i) {
+        if (order_bits(group_max[i / per_group][threadIdx.x]) < least) continue;
+        for (int j = 0; j < kU; ++j) {
+          const int v = u0 + (i * kU + j) * kT + threadIdx.x;
+          if (v >= u1) break;
+          float f[V];
+          Vec16<T>::unpack(__ldg(units + v), f);
+#pragma unroll
+          for (int n = 0; n < V; ++n) hold(f[n], row.col(v) + n);
+        }
+      }
+      if (single >= 0) hold(group_max[kGroups][threadIdx.x], single);
+    }
+    __syncthreads();
+    if (count <= kHeld) {
+      rank_keys(held, count, k, best);
+    } else {
+      unsigned long long last = ~0ull;
+      for (int i = 0; i < k; ++i) {
+        unsigned long long next = 0ull;
+        auto see = [&](float v, int c) {
+          const unsigned long long key = order_key(v, uint32_t(c));
+          if (key < last && key > next) next = key;
+        };
+        for (int v = u0 + threadIdx.x; v < u1; v += kT) {
+          float f[V];
+          Vec16<T>::unpack(__ldg(units + v), f);
+#pragma unroll
+          for (int n = 0; n < V; ++n) see(f[n], row.col(v) + n);
+        }
+        if (single >= 0) see(to_f32(row.x[single]), single);
+        last = block_fold(next, redk, Max());
+        if (threadIdx.x == 0) best[i] = last;
+      }
+    }
+  }
+
+  Part all;
+  if (ranks == 1) {
+    __syncthreads();
+    all = part;
+  } else {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (rank == 0) {
+      all = part;
+      for (int j = 1; j < ranks; ++j) all.max = fmaxf(all.max, cluster.map_shared_rank(&part, j)->max);
+      const float to = all.max;
+      all.sum = all.dot = 0.0;
+      for (int j = 0; j < ranks; ++j) {
+        const Part o = *cluster.map_shared_rank(&part, j);
+        const float by = below(o.max, to, s), e = exp2_approx(by);
+        all.sum += o.sum * e;
+        all.dot += (o.dot + by * o.sum) * e;
+      }
+      if constexpr (kTop)
+        for (int i = threadIdx.x; i < ranks * k; i += kT) held[i] = cluster.map_shared_rank(best, i / k)[i % k];
+    }
+    cluster.sync();  // the other parts are read
+    if (rank != 0) return;
+    if constexpr (kTop) {
+      // A part with fewer than k elements has zeros after them, which are no keys: they rank last.
+      __syncthreads();
+      rank_keys(held, ranks * k, k, best);
+      __syncthreads();
+    }
+  }
+  const bool none = all.max == -CUDART_INF_F && all.sum == 0.0;  // every logit is -inf
+  const bool bad = !(all.sum < CUDART_INF);
+  const float ln_sum = none ? -CUDART_INF_F : log1pf(float(all.sum - 1.0));
+  const float m0 = none ? 0.f : all.max;
+  if (threadIdx.x == 0) {
+    float lp = CUDART_NAN_F;
+    if (target >= 0 && target < vocab) lp = none ? -CUDART_INF_F : fmaf(given - m0, inv_temp, -ln_sum);
+    else record_device_error(DORA_ERR_INVALID_ARGUMENT);
+    logprobs[r] = lp;
+    lse[r] = none ? -CUDART_INF_F : fmaf(m0, inv_temp, ln_sum);
+    if constexpr (kEntropy) entropy[r] = none ? 0.f : ln_sum - kLn2 * float(all.dot / all.sum);
+  }
+  if constexpr (kTop)
+    for (int i = threadIdx.x; i < k; i += kT) {
+      top_lp[r * k + i] = bad ? CUDART_NAN_F : none ? -CUDART_INF_F : fmaf(key_value(best[i]) - m0, inv_temp, -ln_sum);
+      top_idx[r * k + i] = bad ? i : key_col(best[i]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Backward: one pass, a CTA to a part of a row; bound by HBM.  The units are those of the
+// output; where the logits' rows stand differently to 16 bytes, each is cut out of two of theirs.
+// ---------------------------------------------------------------------------
+// V elements from column c on: c's 16-byte unit and the one after it, shifted by `off` elements.
+template <typename T> __device__ __forceinline__ uint4 cut(const uint4& a, const uint4& b, int off) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t o[5];
+  switch (sizeof(T) == 4 ? off : off / 2) {  // the same for the whole row
+    case 0: for (int i = 0; i < 5; ++i) o[i] = w[i]; break;
+    case 1: for (int i = 0; i < 5; ++i) o[i] = w[i + 1]; break;
+    case 2: for (int i = 0; i < 5; ++i) o[i] = w[i + 2]; break;
+    default: for (int i = 0; i < 5; ++i) o[i] = w[i + 3]; break;
+  }
+  if (sizeof(T) == 2 && (off & 1))
+    for (int i = 0; i < 4; ++i) o[i] = __byte_perm(o[i], o[i + 1], 0x5432);
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kT)
 logprobs_bwd_kernel(const T* logits, int64_t ld, const int64_t* __restrict__ targets, int64_t ignore, float s,
                     float inv_temp, const float* __restrict__ lse, const float* __restrict__ entropy,
                     const float* __restrict__ g_lp, const float* __restrict__ g_ent, const float* __restrict__ g_lse,
-                    T* d, int64_t ldd, int64_t rows, int64_t vocab) {
+                    T* d, int64_t ldd, int vocab, int parts) {
+  constexpr int V = Vec16<T>::N, N = V / 2;
   __shared__ float red[kT / 32];
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t target = targets[r];
-    const T* x = logits + r * ld;
-    T* o = d + r * ldd;
-    float L = lse[r];
-    if (target == ignore || L == -CUDART_INF_F) {
-      for (int64_t c = threadIdx.x; c < vocab; c += kT) o[c] = from_f32<T>(0.f);
-      continue;
+  const int64_t r = blockIdx.x / parts;
+  const int part = blockIdx.x % parts;
+  const int64_t target = targets[r];
+  const T* x = logits + r * ld;
+  const Row<T> out(d + r * ldd, vocab);
+  T* o = d + r * ldd;
+  const int u0 = int(int64_t(out.units) * part / parts), u1 = int(int64_t(out.units) * (part + 1) / parts);
+  const int single = out.single(part == 0, part == parts - 1);
+  float L = lse[r];
+  if (target == ignore || L == -CUDART_INF_F) {
+    for (int u = u0 + threadIdx.x; u < u1; u += kT) st_stream(o + out.col(u), make_uint4(0, 0, 0, 0));
+    if (single >= 0) o[single] = from_f32<T>(0.f);
+    return;
+  }
+  float m = 0.f;  // log p_j = (x_j - m) / T - L
+  if (fabsf(L) > kWideLse) {
+    // The row in place of which the gradient is written may be partly overwritten by now, by another CTA: the launch
+    // gives rows one CTA each then.
+    m = -CUDART_INF_F;
+    for (int c = threadIdx.x; c < vocab; c += kT) m = fmaxf(m, to_f32(x[c]));
+    m = block_fold(m, red, Max());
+    float sum = 0.f;
+    for (int c = threadIdx.x; c < vocab; c += kT) sum += exp2_approx((to_f32(x[c]) - m) * s);
+    L = logf(block_fold(sum, red, Sum()));
+  }
+  const float glp = g_lp ? g_lp[r] : 0.f, gl = g_lse ? g_lse[r] : 0.f, ge = kEntropy ? g_ent[r] : 0.f;
+  // dx_j = p_j (a + b log p_j) + 1[j = t] g_lp / T
+  const float a = (gl - glp - (kEntropy ? ge * entropy[r] : 0.f)) * inv_temp, b = -ge * inv_temp;
+  auto slope = [&](Two v) {
+    const Two lp = fma2(add2(v, both(-m)), both(inv_temp), both(-L));
+    const Two t = mul2(lp, both(kLog2e));
+    const Two p{exp2_approx(t.a), exp2_approx(t.b)};
+    if constexpr (!kEntropy) return mul2(p, both(a));
+    return mul2(p, fma2(both(b), Two{fmaxf(lp.a, -200.f), fmaxf(lp.b, -200.f)}, both(a)));
+  };
+  const int off = int((reinterpret_cast<uintptr_t>(x + out.head) & 15) / sizeof(T));  // of the logits' row there
+  auto finish = [&](int u, const uint4& q) {
+    Two f[N];
+    Pairs<T>::unpack(q, f);
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = slope(f[n]);
+    const int64_t at = target - out.col(u);
+    if (at >= 0 && at < V) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (at == 2 * n) f[n].a = fmaf(glp, inv_temp, f[n].a);
+        if (at == 2 * n + 1) f[n].b = fmaf(glp, inv_temp, f[n].b);
+      }
     }
-    float m = 0.f;  // log p_j = (x_j - m) / T - L
-    if (fabsf(L) > kWideLse) {
-      m = -CUDART_INF_F;
-      for (int64_t c = threadIdx.x; c < vocab; c += kT) m = fmaxf(m, to_f32(x[c]));
-      m = block_fold(m, red, Max());
-      float sum = 0.f;
-      for (int64_t c = threadIdx.x; c < vocab; c += kT) sum += exp2_approx((to_f32(x[c]) - m) * s);
-      L = logf(block_fold(sum, red, Sum()));
+    st_stream(o + out.col(u), Pairs<T>::pack(f));
+  };
+  if (off == 0) {
+    for (int u = u0 + threadIdx.x; u < u1; u += kT * kU) {
+      uint4 q[kU];
+#pragma unroll
+      for (int j = 0; j < kU; ++j)
+        if (u + j * kT < u1) q[j] = ld_stream_coherent(x + out.col(u + j * kT));
+#pragma unroll
+      for (int j = 0; j < kU; ++j)
+        if (u + j * kT < u1) finish(u + j * kT, q[j]);
     }
-    const float glp = g_lp ? g_lp[r] : 0.f, gl = g_lse ? g_lse[r] : 0.f, ge = g_ent ? g_ent[r] : 0.f;
-    // dx_j = p_j (a + b log p_j) + 1[j = t] g_lp / T
-    const float a = (gl - glp - (g_ent ? ge * entropy[r] : 0.f)) * inv_temp, b = -ge * inv_temp;
-    for (int64_t c = threadIdx.x; c < vocab; c += kT) {
-      const float lp = fmaf(to_f32(x[c]) - m, inv_temp, -L);
-      float v = exp2_approx(lp * kLog2e) * fmaf(b, fmaxf(lp, -200.f), a);
-      if (c == target) v = fmaf(glp, inv_temp, v);
-      o[c] = from_f32<T>(v);
+  } else {
+    for (int u = u0 + threadIdx.x; u < u1; u += kT) {
+      const T* from = x + out.col(u) - off;  // a multiple of 16
+      uint4 q;
+      if (from >= x && out.col(u) - off + 2 * V <= vocab) {
+        q = cut<T>(__ldg(reinterpret_cast<const uint4*>(from)), __ldg(reinterpret_cast<const uint4*>(from + V)), off);
+      } else {  // a unit that reaches out of the row
+        T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int n = 0; n < V; ++n) e[n] = x[out.col(u) + n];
+      }
+      finish(u, q);
     }
+  }
+  if (single >= 0) {
+    float v = slope(both(to_f32(x[single]))).a;
+    if (single == target) v = fmaf(glp, inv_temp, v);
+    o[single] = from_f32<T>(v);
   }
 }
 
-unsigned row_grid(int64_t rows) { return unsigned(rows < (1 << 20) ? rows : (1 << 20)); }
+// Parts of a row: enough that `want` CTAs run, each with at least `least` 16-byte units; powers of two.
+int row_parts(int64_t rows, int64_t units, int64_t want, int64_t least, int most) {
+  int n = 1;
+  while (n < most && rows * n * 2 <= want && units / (2 * n) >= least) n *= 2;
+  return n;
+}
 
 bool args_ok(int64_t rows, int64_t vocab, int64_t ld, double temperature, int dtype) {
   return rows >= 0 && vocab >= 1 && vocab < (int64_t(1) << 31) && ld >= vocab && rows <= (int64_t(1) << 40) &&
@@ -205,11 +513,29 @@ extern "C" int dora_token_logprobs_fwd(const void* logits, int64_t ld, const voi
   const float s = float(1.4426950408889634074 / temperature), inv_temp = float(1.0 / temperature);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    logprobs_fwd_kernel<T><<<row_grid(rows), kT, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const T*>(logits), ld, static_cast<const int64_t*>(targets), ignore_index, s, inv_temp,
-        static_cast<float*>(logprobs), static_cast<float*>(lse), static_cast<float*>(entropy), top_k,
-        static_cast<float*>(top_logprobs), static_cast<int64_t*>(top_indices), rows, vocab);
-    return check_launch();
+    // A cluster of up to eight CTAs to a row while that makes no more than three CTAs an SM, each with a round of work.
+    const int ranks = row_parts(rows, vocab / Vec16<T>::N, int64_t(num_sms()) * 3, kT * kU / 2, 8);
+    if (rows * ranks > 0x7fffffff) return int(DORA_ERR_UNSUPPORTED);
+    auto go = [&](auto kernel) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(unsigned(rows * ranks));
+      cfg.blockDim = dim3(kT);
+      cfg.stream = static_cast<cudaStream_t>(stream);
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = unsigned(ranks);
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      count_launches(1);
+      const cudaError_t e = cudaLaunchKernelEx(
+          &cfg, kernel, static_cast<const T*>(logits), ld, static_cast<const int64_t*>(targets), ignore_index, s,
+          inv_temp, static_cast<float*>(logprobs), static_cast<float*>(lse), static_cast<float*>(entropy), top_k,
+          static_cast<float*>(top_logprobs), static_cast<int64_t*>(top_indices), int(vocab), ranks);
+      return e == cudaSuccess ? int(DORA_OK) : set_cuda_error(e);
+    };
+    if (top_k) return entropy ? go(logprobs_fwd_kernel<T, true, true>) : go(logprobs_fwd_kernel<T, false, true>);
+    return entropy ? go(logprobs_fwd_kernel<T, true, false>) : go(logprobs_fwd_kernel<T, false, false>);
   });
 }
 
@@ -225,11 +551,17 @@ extern "C" int dora_token_logprobs_bwd(const void* logits, int64_t ld, const voi
   const float s = float(1.4426950408889634074 / temperature), inv_temp = float(1.0 / temperature);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    logprobs_bwd_kernel<T><<<row_grid(rows), kT, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const T*>(logits), ld, static_cast<const int64_t*>(targets), ignore_index, s,
-        inv_temp, static_cast<const float*>(lse), static_cast<const float*>(entropy),
-        static_cast<const float*>(g_logprobs), static_cast<const float*>(g_entropy), static_cast<const float*>(g_lse),
-        static_cast<T*>(d_logits), ld_d, rows, vocab);
-    return check_launch();
+    // Parts of at least four rounds while there are few CTAs; one in place of the logits (see the kernel).
+    const int parts = logits == d_logits ? 1 : row_parts(rows, vocab / Vec16<T>::N, int64_t(num_sms()) * 8, kT * kU, 64);
+    if (rows * parts > 0x7fffffff) return int(DORA_ERR_UNSUPPORTED);
+    auto go = [&](auto kernel) {
+      kernel<<<unsigned(rows * parts), kT, 0, static_cast<cudaStream_t>(stream)>>>(
+          static_cast<const T*>(logits), ld, static_cast<const int64_t*>(targets), ignore_index, s, inv_temp,
+          static_cast<const float*>(lse), static_cast<const float*>(entropy), static_cast<const float*>(g_logprobs),
+          static_cast<const float*>(g_entropy), static_cast<const float*>(g_lse), static_cast<T*>(d_logits), ld_d,
+          int(vocab), parts);
+      return check_launch();
+    };
+    return g_entropy ? go(logprobs_bwd_kernel<T, true>) : go(logprobs_bwd_kernel<T, false>);
   });
 }
