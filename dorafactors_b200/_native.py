@@ -446,9 +446,10 @@ def addr(t: torch.Tensor | None) -> int | None:
 def rows_of(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """``x`` as rows of its last dimension: (tensor that holds the data, rows, cols, row
     stride).  Rows of a wider buffer are taken as they are; other layouts are copied."""
-    cols = x.shape[-1]
+    shape = x.shape
+    cols = shape[-1]
     if x.is_contiguous():
-        return x, x.numel() // cols if cols else x.shape[:-1].numel(), cols, cols
+        return x, x.numel() // cols if cols else shape[:-1].numel(), cols, cols
     if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
         return x, x.shape[0], cols, x.stride(0)
     if x.ndim > 2 and x.stride(-1) == 1 and x.numel():

@@ -59,8 +59,8 @@ def _forward(logits, targets, temperature, entropy, top_k, ignore_index):
     data, rows, vocab, ld = _native.rows_of(logits)
     dev, shape = logits.device, targets.shape
     lp = torch.empty(shape, dtype=torch.float32, device=dev)
-    lse = torch.empty(shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
+    lse = torch.empty_like(lp)
+    ent = torch.empty_like(lp) if entropy else None
     top = idx = None
     if top_k:
         top = torch.empty((*shape, top_k), dtype=torch.float32, device=dev)
@@ -143,4 +143,6 @@ def token_logprobs(logits, targets, *, temperature: float = 1.0, entropy: bool =
     vocabulary gives a NaN log probability and sets the device error word
     (``_native.device_error``).
     """
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, float(temperature), entropy, int(top_k), ignore_index))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, float(temperature), entropy, int(top_k), ignore_index))
+    return TokenLogprobs(*_forward(logits, targets, float(temperature), entropy, int(top_k), ignore_index))

@@ -6,6 +6,9 @@
     python -m dorafactors_b200.microbench --op linear_output_bwd --rows 16384 --cols 28672
     python -m dorafactors_b200.microbench --op allgather:2 --rows 32768 --cols 14336
     python -m dorafactors_b200.microbench --op sweep      # rank sweep on an 8192 x 8192 layer
+    python -m dorafactors_b200.microbench --op layer_norm_bwd --rows 16384 --cols 8192   # or rms_norm_*, *_fwd
+    python -m dorafactors_b200.microbench --op logprobs_fwd --rows 4096 --cols 128256 --top-k 5
+    python -m dorafactors_b200.microbench --op adamw --tensors 672 --cols 524288 --state-bits 8
 
 Each run prints one JSON line per measurement: average milliseconds per call,
 the algorithmic work, achieved GB/s or TFLOP/s and the fraction of the measured
@@ -129,11 +132,64 @@ def bench_compose(op: str, rows: int, cols: int, iters: int, warmup: int, dtype=
             "hbm_frac": gbs / pk["hbm_gbs"], "peak_source": pk["source"]}
 
 
+def bench_norm_layer(op: str, rows: int, cols: int, iters: int, warmup: int, dtype=torch.bfloat16) -> dict:
+    """layer_norm_fwd | layer_norm_bwd | rms_norm_fwd | rms_norm_bwd, weights in ``dtype``."""
+    from . import norms
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, dy = (torch.randn(rows, cols, device="cuda", generator=g).to(dtype) for _ in range(2))
+    w, b = (torch.randn(cols, device="cuda", generator=g).to(dtype) for _ in range(2))
+    if op.startswith("layer"):
+        _, mean, rstd = norms.layer_norm_forward(x, w, b)
+        fwd, bwd = lambda: norms.layer_norm_forward(x, w, b), lambda: norms.layer_norm_backward(dy, x, w, mean, rstd)
+    else:
+        _, rstd = norms.rms_norm_forward(x, w)
+        fwd, bwd = lambda: norms.rms_norm_forward(x, w), lambda: norms.rms_norm_backward(dy, x, w, rstd)
+    ms = _time(fwd if op.endswith("fwd") else bwd, iters, warmup)
+    return _hbm_line(op, ms, (2 if op.endswith("fwd") else 3) * x.element_size() * rows * cols, rows=rows, cols=cols)
+
+
+def bench_logprobs(op: str, rows: int, vocab: int, top_k: int, iters: int, warmup: int, dtype=torch.bfloat16) -> dict:
+    """logprobs_fwd (with entropy and ``top_k`` alternatives) | logprobs_bwd."""
+    from .logprobs import token_logprobs, token_logprobs_backward
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = (torch.randn(rows, vocab, device="cuda", generator=g) * 3).to(dtype)
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    r = token_logprobs(x, t, entropy=True)
+    if op == "logprobs_fwd":
+        ms = _time(lambda: token_logprobs(x, t, entropy=True, top_k=top_k), iters, warmup)
+    else:
+        ms = _time(lambda: token_logprobs_backward(r.logprobs, r.entropy, None, x, t, r.logsumexp, r.entropy), iters, warmup)
+    return _hbm_line(op, ms, (1 if op == "logprobs_fwd" else 2) * x.element_size() * rows * vocab, rows=rows, vocab=vocab,
+                     top_k=top_k)
+
+
+def bench_adamw(tensors: int, numel: int, bits: int, iters: int, warmup: int, dtype=torch.bfloat16) -> dict:
+    from .optim import AdamW
+
+    params = [torch.nn.Parameter(torch.zeros(numel, device="cuda", dtype=dtype)) for _ in range(tensors)]
+    for p in params:
+        p.grad = torch.randn(numel, device="cuda").to(dtype)
+    opt = AdamW(params, state_bits=bits)
+    ms = _time(opt.step, iters, warmup)
+    per = 3 * params[0].element_size() + (16 if bits == 32 else 4 + 16 / 256)
+    return _hbm_line("adamw", ms, per * tensors * numel, tensors=tensors, numel=numel, state_bits=bits)
+
+
+def _hbm_line(op: str, ms: float, nbytes: float, **shape) -> dict:
+    pk = _peaks()
+    gbs = nbytes / (ms * 1e-3) / 1e9
+    return {"op": op, **shape, "ms": ms, "bytes": nbytes, "gbs": gbs, "hbm_frac": gbs / pk["hbm_gbs"],
+            "peak_source": pk["source"]}
+
+
 def main(argv=None) -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--op", required=True,
                     help="norm | compose_fwd | compose_fwd_inference | compose_bwd | linear_output_fwd | "
-                         "linear_output_bwd | allgather[:ranks] | sweep")
+                         "linear_output_bwd | allgather[:ranks] | sweep | layer_norm_fwd | layer_norm_bwd | "
+                         "rms_norm_fwd | rms_norm_bwd | logprobs_fwd | logprobs_bwd | adamw")
     ap.add_argument("--out", type=int, default=28672)
     ap.add_argument("--in", dest="inp", type=int, default=8192)
     ap.add_argument("--rank", type=int, default=384)
@@ -141,6 +197,9 @@ def main(argv=None) -> None:
     ap.add_argument("--cols", type=int, default=28672)
     ap.add_argument("--adapter-dtype", choices=["same", "fp32"], default="same",
                     help="norm: adapters in the weight dtype or in fp32 (PEFT's default on a bf16 base)")
+    ap.add_argument("--top-k", type=int, default=0, help="logprobs_fwd: alternatives")
+    ap.add_argument("--tensors", type=int, default=672, help="adamw: tensors of --cols elements")
+    ap.add_argument("--state-bits", type=int, default=32, choices=(8, 32), help="adamw: moments")
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
     a = ap.parse_args(argv)
@@ -153,6 +212,12 @@ def main(argv=None) -> None:
             print(json.dumps(bench_norm(8192, 8192, r, a.iters, a.warmup)), flush=True)
         for op in ("compose_fwd", "compose_bwd"):
             print(json.dumps(bench_compose(op, 8192, 8192, a.iters, a.warmup)), flush=True)
+    elif a.op in ("layer_norm_fwd", "layer_norm_bwd", "rms_norm_fwd", "rms_norm_bwd"):
+        print(json.dumps(bench_norm_layer(a.op, a.rows, a.cols, a.iters, a.warmup)), flush=True)
+    elif a.op in ("logprobs_fwd", "logprobs_bwd"):
+        print(json.dumps(bench_logprobs(a.op, a.rows, a.cols, a.top_k, a.iters, a.warmup)), flush=True)
+    elif a.op == "adamw":
+        print(json.dumps(bench_adamw(a.tensors, a.cols, a.state_bits, a.iters, a.warmup)), flush=True)
     else:
         print(json.dumps(bench_compose(a.op, a.rows, a.cols, a.iters, a.warmup)), flush=True)
     if _native.device_error(reset=True) != 0:

@@ -21,47 +21,54 @@ from torch.autograd.function import once_differentiable
 from . import _native
 
 
-def _vector(v, cols: int, name: str, what: str):
-    if v.ndim != 1 or v.shape[0] != cols:
-        raise ValueError(f"{what}: {name} {tuple(v.shape)} does not match the last dimension {cols}")
-
-
-def _params(x, weight, bias, what: str):
+def _params(x, cols: int, weight, bias, what: str):
     """Checked operands: (weight, bias, their dtype code)."""
-    if x.ndim == 0:
-        raise ValueError(f"{what}: the input must have at least one dimension")
-    _native.require_cuda(x, weight, bias, what=what)
-    cols, act = x.shape[-1], _native.dtype_code(x)
-    wdt = None
+    if not x.is_cuda:
+        _native.require_cuda(x, what=what)
+    act = _native.DTYPE_CODE.get(x.dtype)
+    if act is None:
+        _native.dtype_code(x)
+    dtype = None
     for v, name in ((weight, "weight"), (bias, "bias")):
         if v is not None:
-            _vector(v, cols, name, what)
-            wdt = v.dtype if wdt in (None, v.dtype) else torch.float32
-    if wdt is None:
+            if v.shape != (cols,):
+                raise ValueError(f"{what}: {name} {tuple(v.shape)} does not match the last dimension {cols}")
+            if v.get_device() != x.get_device():
+                _native.require_cuda(x, v, what=what)
+            dtype = v.dtype if dtype in (None, v.dtype) else torch.float32
+    if dtype is None:
         return None, None, act
-    if wdt is not x.dtype:
-        wdt = torch.float32
-    weight = weight if weight is None or (weight.dtype is wdt and weight.is_contiguous()) else weight.to(wdt).contiguous()
-    bias = bias if bias is None or (bias.dtype is wdt and bias.is_contiguous()) else bias.to(wdt).contiguous()
-    return weight, bias, _native.DTYPE_CODE[wdt]
+    if dtype is not x.dtype:
+        dtype = torch.float32
+    if weight is not None and not (weight.dtype is dtype and weight.is_contiguous()):
+        weight = weight.to(dtype).contiguous()
+    if bias is not None and not (bias.dtype is dtype and bias.is_contiguous()):
+        bias = bias.to(dtype).contiguous()
+    return weight, bias, _native.DTYPE_CODE[dtype]
 
 
 def _forward(x, weight, bias, eps, rms: bool, what: str):
-    w, b, code = _params(x, weight, bias, what)
+    shape = x.shape
+    if not shape:
+        raise ValueError(f"{what}: the input must have at least one dimension")
     if not eps >= 0:
         raise ValueError(f"{what}: eps must not be negative, got {eps}")
+    w, b, code = _params(x, shape[-1], weight, bias, what)
     data, rows, cols, ld = _native.rows_of(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    lead = x.shape[:-1]
-    rstd = torch.empty(lead, dtype=torch.float32, device=x.device)
-    mean = None if rms else torch.empty(lead, dtype=torch.float32, device=x.device)
+    device = x.device
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    lead = shape[:-1]
+    rstd = torch.empty(lead, dtype=torch.float32, device=device)
+    mean = None if rms else torch.empty(lead, dtype=torch.float32, device=device)
     if rows and cols:
         _native.layer_norm_fwd(data, rows, cols, ld, w, b, code, eps, y, mean, rstd, rms)
     return y, mean, rstd
 
 
 def _backward(dy, x, weight, mean, rstd, need, rms: bool, what: str, bias_dtype=None):
-    w, _, code = _params(x, weight, None, what)
+    if not x.ndim:
+        raise ValueError(f"{what}: the input must have at least one dimension")
+    w, _, code = _params(x, x.shape[-1], weight, None, what)
     if dy.shape != x.shape:
         raise ValueError(f"{what}: dy {tuple(dy.shape)} and x {tuple(x.shape)} differ in shape")
     _native.require_cuda(x, dy, mean, rstd, what=what)
@@ -130,14 +137,22 @@ class _Norm(torch.autograd.Function):
         return dx, dw, db, None, None
 
 
+def _tracked(x, weight, bias) -> bool:
+    return x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
+
+
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension."""
-    return _Norm.apply(x, weight, bias, eps, False)
+    if torch.is_grad_enabled() and _tracked(x, weight, bias):
+        return _Norm.apply(x, weight, bias, eps, False)
+    return _forward(x, weight, bias, eps, False, "layer_norm")[0]
 
 
 def rms_norm(x, weight=None, eps: float = 1e-6) -> torch.Tensor:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension."""
-    return _Norm.apply(x, weight, None, eps, True)
+    if torch.is_grad_enabled() and _tracked(x, weight, None):
+        return _Norm.apply(x, weight, None, eps, True)
+    return _forward(x, weight, None, eps, True, "rms_norm")[0]
 
 
 class LayerNorm(nn.Module):

@@ -206,7 +206,6 @@ class AdamW(torch.optim.Optimizer):
         _native.adamw_step(address, len(table), g.dtype, g.bits, float(group["lr"]), group["betas"], group["eps"],
                            group["weight_decay"], step, g.device)
 
-    @torch.no_grad()
     def moments(self, group: int = 0):
         """``(exp_avg, exp_avg_sq)`` of a group as flat fp32 tensors, each parameter at a multiple
         of 256 elements.  With 32-bit state these are the state itself, else decoded copies."""
