@@ -130,6 +130,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n,
   for (int i = threadIdx.x; i < n; i += kT) {
     const unsigned long long mine = keys[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) r += keys[j] > mine;
     if (r < k) out[r] = mine;
   }
@@ -148,8 +149,6 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
   __shared__ Part part;
   __shared__ float group_max[kTop ? kGroups + 1 : 1][kT];  // [kGroups]: the single element
   __shared__ unsigned long long held[kTop ? kHeld : 1], best[kTop ? kMaxTop : 1], redk[kT / 32];
-  __shared__ uint32_t thread_max[kTop ? kT : 1];
-  __shared__ uint32_t bound;
   __shared__ int count;
 
   const int64_t r = blockIdx.x / ranks;
@@ -252,47 +251,48 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
 
   if constexpr (kTop) {
     const bool any = u0 + int(threadIdx.x) < u1 || single >= 0;
-    thread_max[threadIdx.x] = any ? order_bits(m) : 0u;
-    if (threadIdx.x == 0) {
-      bound = 0u;
-      count = 0;
-    }
+    const uint32_t mine = any ? order_bits(m) : 0u;
+    if (threadIdx.x == 0) count = 0;
     if (threadIdx.x < kMaxTop) best[threadIdx.x] = 0ull;
-    __syncthreads();
-    {
-      const uint32_t mine = thread_max[threadIdx.x];
-      int above = 0;
-      const uint4* all = reinterpret_cast<const uint4*>(thread_max);
-      for (int j = 0; j < kT / 4; ++j) {
-        const uint4 o = all[j];
-        above += (o.x > mine || (o.x == mine && 4 * j < int(threadIdx.x))) +
-                 (o.y > mine || (o.y == mine && 4 * j + 1 < int(threadIdx.x))) +
-                 (o.z > mine || (o.z == mine && 4 * j + 2 < int(threadIdx.x))) +
-                 (o.w > mine || (o.w == mine && 4 * j + 3 < int(threadIdx.x)));
-      }
-      if (above == k - 1) bound = mine;
+    // The largest bound of 16 leading bits that at least k threads' maxima reach, bit by bit (all 16 of a 16-bit logit).
+    uint32_t least = 0u;
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t trial = least | (1u << bit);
+      if (__syncthreads_count(mine >= trial) >= k) least = trial;
     }
-    __syncthreads();
-    const uint32_t least = bound;
-    auto hold = [&](float v, int c) {
-      if (order_bits(v) >= least) {
-        const int at = atomicAdd(&count, 1);  // any order: the keys are ranked
-        if (at < kHeld) held[at] = order_key(v, uint32_t(c));
-      }
+    const float reach = least > order_bits(-CUDART_INF_F) ? key_value(static_cast<unsigned long long>(least) << 32) : -CUDART_INF_F;
+    auto hold = [&](int c) {
+      const int at = atomicAdd(&count, 1);  // any order: the keys are ranked
+      if (at < kHeld) held[at] = order_key(to_f32(row.x[c]), uint32_t(c));
     };
-    if (thread_max[threadIdx.x] >= least) {
-      for (int i = 0; i < rounds; ++i) {
-        if (order_bits(group_max[i / per_group][threadIdx.x]) < least) continue;
-        for (int j = 0; j < kU; ++j) {
-          const int v = u0 + (i * kU + j) * kT + threadIdx.x;
-          if (v >= u1) break;
-          float f[V];
-          Vec16<T>::unpack(__ldg(units + v), f);
+    if (mine >= least) {
+      uint32_t wanted = 0u;  // groups that reach the bound
 #pragma unroll
-          for (int n = 0; n < V; ++n) hold(f[n], row.col(v) + n);
+      for (int g = 0; g < kGroups; ++g)
+        if (g * per_group < rounds && order_bits(group_max[g][threadIdx.x]) >= least) wanted |= 1u << g;
+      for (int i = 0; i < rounds && wanted; ++i) {
+        const int g = i / per_group;
+        if (!(wanted >> g & 1u)) continue;
+        if (i + 1 == (g + 1) * per_group) wanted &= ~(1u << g);
+        const int v = u0 + i * kU * kT + threadIdx.x;
+        uint4 again[kU];
+#pragma unroll
+        for (int j = 0; j < kU; ++j)
+          again[j] = v + j * kT < u1 ? __ldg(units + v + j * kT) : no_logits<T>();
+        uint32_t reached = 0u;
+#pragma unroll
+        for (int j = 0; j < kU; ++j) {
+          float f[V];
+          Vec16<T>::unpack(again[j], f);
+#pragma unroll
+          for (int n = 0; n < V; ++n) reached |= v + j * kT < u1 && f[n] >= reach ? 1u << (j * V + n) : 0u;
+        }
+        for (; reached; reached &= reached - 1) {
+          const int e = __ffs(int(reached)) - 1;
+          hold(row.col(v + e / V * kT) + e % V);
         }
       }
-      if (single >= 0) hold(group_max[kGroups][threadIdx.x], single);
+      if (single >= 0 && group_max[kGroups][threadIdx.x] >= reach) hold(single);
     }
     __syncthreads();
     if (count <= kHeld) {
