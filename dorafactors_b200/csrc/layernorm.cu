@@ -16,7 +16,8 @@ namespace dora {
 namespace {
 
 constexpr int kT = 256;       // threads of the kernels for any width
-constexpr int kFwdFill = 768, kBwdFill = 512;
+constexpr int kBwdFill = 512;
+constexpr int fwd_fill(bool params_in_shared) { return params_in_shared ? 512 : 768; }
 
 // ---------------------------------------------------------------------------
 // A row and the threads that share it.  `tpr` threads hold a row: up to 32 (a power of
@@ -141,14 +142,18 @@ __device__ __forceinline__ Walk walk(int64_t rows, int tpr, int groups) {
 }
 
 // Forward: the variance is taken around the mean, from the registers.
-// kParams: 0 none, 1 a weight, 2 a weight and a bias, of type TW; they come from L1 for each row.
+// kParams: 0 none, 1 a weight, 2 a weight and a bias, of type TW.  They stand in shared memory, each thread's units in
+// places of its own, so two CTAs of 128 registers a thread run on an SM; fp32 ones of 16-bit rows, which would take twice
+// the room, come from L1 for each row, with three CTAs of 80.  (bf16, 16384 x 8192, with weight and bias: 90 us; from L1
+// with three CTAs 101 us, with two 112 us; in registers 109 us.)
 template <typename TA, typename TW, bool kRms, int kParams, int PER, int S, int kMax>
-__global__ void __launch_bounds__(kMax, kFwdFill / kMax)
+__global__ void __launch_bounds__(kMax, fwd_fill(sizeof(TW) == sizeof(TA)) / kMax)
 ln_fwd_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w, const void* __restrict__ b, float eps, TA* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
               int cols, int tpr, int groups) {
   using P = Pairs<TA>;
   constexpr int N = P::N, V = 2 * N;
-  extern __shared__ uint4 ring[];  // [S][PER][threads]
+  constexpr bool kShared = sizeof(TW) == sizeof(TA);
+  extern __shared__ uint4 ring[];  // [S][PER][threads], then the parameters: [kParams][PER][threads]
   DORA_ROW_SUM(sum, kMax, 1);
   const Walk at = walk(rows, tpr, groups);
   const float inv = 1.0f / float(cols);
@@ -173,6 +178,17 @@ ln_fwd_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w,
   };
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) fetch();
+  uint4* held = ring + S * PER * blockDim.x + threadIdx.x;
+  if constexpr (kShared && kParams > 0) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (has[p]) {
+        const int c = (p * tpr + at.t) * V;
+        held[p * blockDim.x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const TA*>(w) + c));
+        if constexpr (kParams > 1)
+          held[(PER + p) * blockDim.x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const TA*>(b) + c));
+      }
+  }
   int s = 0;
   for (int64_t k = 0; k < at.rounds; ++k) {
     fetch();
@@ -219,12 +235,14 @@ ln_fwd_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w,
 #pragma unroll
           for (int i = 0; i < N; ++i) o[i] = mul2(f[p][i], both(rs));
           if constexpr (kParams > 0) {
-            load_param<TA, TW>(w, (p * tpr + at.t) * V, v);
+            if constexpr (kShared) P::unpack(held[p * blockDim.x], v);
+            else load_param<TA, TW>(w, (p * tpr + at.t) * V, v);
 #pragma unroll
             for (int i = 0; i < N; ++i) o[i] = mul2(o[i], v[i]);
           }
           if constexpr (kParams > 1) {
-            load_param<TA, TW>(b, (p * tpr + at.t) * V, v);
+            if constexpr (kShared) P::unpack(held[(PER + p) * blockDim.x], v);
+            else load_param<TA, TW>(b, (p * tpr + at.t) * V, v);
 #pragma unroll
             for (int i = 0; i < N; ++i) o[i] = add2(o[i], v[i]);
           }
@@ -769,16 +787,15 @@ int64_t walkers(const Shape& s, int64_t rows, int per_sm, bool fwd) {
   if (!fwd && n > num_sms() && n > need / 8) n = need / 8 > num_sms() ? need / 8 : num_sms();
   return n < 1 ? 1 : n;
 }
-// 16-byte units: 80 registers a thread in the forward (768 threads an SM), 128 in the backward (512; 64 for rows
-// of more than 1024 units).
-Plan plan_units(int64_t rows, int64_t units, bool fwd) {
+// 16-byte units; `fill` threads an SM have the registers that the kernels take.
+Plan plan_units(int64_t rows, int64_t units, bool fwd, int fill) {
   Plan p;
   p.per = fwd ? (units <= 768 * 4 ? 4 : 0) : units <= 2048 ? 2 : 0;
   if (!p.per) return p;
   p.shape = share_row(units, p.per, 128);
   if (fwd) p.most = p.shape.groups > 1 ? 128 : p.shape.threads > 256 ? 768 : 256;
   else p.most = p.shape.groups > 1 ? 128 : units > 1024 ? 1024 : 512;
-  p.ctas = walkers(p.shape, rows, (fwd ? kFwdFill : kBwdFill) / p.shape.threads, fwd);
+  p.ctas = walkers(p.shape, rows, fill / p.shape.threads, fwd);
   return p;
 }
 // Elements, with `buffers` rows in shared memory (200 KB of it an SM).
@@ -807,12 +824,12 @@ int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, bool f3
                float* rstd, int64_t rows, int64_t cols, cudaStream_t st) {
   constexpr int V = Vec16<TA>::N;
   const bool vec = cols % V == 0 && ldx % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
-  const Plan p = vec ? plan_units(rows, cols / V, true) : Plan();
+  const Plan p = vec ? plan_units(rows, cols / V, true, fwd_fill(f32 == (sizeof(TA) == 4))) : Plan();
   auto X = static_cast<const TA*>(x);
   auto Y = static_cast<TA*>(y);
   if (p.per && vec && (w || !b)) {
-    auto go = [&](auto kernel, int S) {
-      const size_t smem = size_t(S) * p.per * p.shape.threads * 16;
+    auto go = [&](auto kernel, int buffers) {
+      const size_t smem = size_t(buffers) * p.per * p.shape.threads * 16;
       const int e = allow_shared(kernel, smem);
       if (e) return e;
       kernel<<<unsigned(p.ctas), p.shape.threads, smem, st>>>(X, ldx, w, b, eps, Y, mean, rstd, rows, int(cols),
@@ -821,10 +838,11 @@ int launch_fwd(const void* x, int64_t ldx, const void* w, const void* b, bool f3
     };
     auto sized = [&](auto tw, auto kind) {
       using TW = decltype(tw);
-      constexpr int K = decltype(kind)::value;
-      if (p.most == 128) return go(ln_fwd_kernel<TA, TW, kRms, K, 4, 4, 128>, 4);
-      return p.most == 256 ? go(ln_fwd_kernel<TA, TW, kRms, K, 4, 4, 256>, 4)
-                           : go(ln_fwd_kernel<TA, TW, kRms, K, 4, 3, 768>, 3);
+      constexpr int K = decltype(kind)::value, more = sizeof(TW) == sizeof(TA) ? K : 0;
+      constexpr int S = sizeof(TW) == sizeof(TA) ? 4 : 3;
+      if (p.most == 128) return go(ln_fwd_kernel<TA, TW, kRms, K, 4, S, 128>, S + more);
+      return p.most == 256 ? go(ln_fwd_kernel<TA, TW, kRms, K, 4, S, 256>, S + more)
+                           : go(ln_fwd_kernel<TA, TW, kRms, K, 4, 2, 768>, 2 + more);
     };
     auto typed = [&](auto tw) {
       if constexpr (!kRms)
@@ -867,7 +885,7 @@ int launch_bwd_rows(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
   constexpr int V = Vec16<TA>::N;
   const bool vec = cols % V == 0 && ldx % V == 0 && lddy % V == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) &&
                    aligned16(w);
-  const Plan p = vec ? plan_units(rows, cols / V, false) : Plan();
+  const Plan p = vec ? plan_units(rows, cols / V, false, kBwdFill) : Plan();
   auto D = static_cast<const TA*>(dy);
   auto X = static_cast<const TA*>(x);
   auto DX = static_cast<TA*>(dx);
@@ -917,7 +935,7 @@ int launch_bwd_rows(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
 size_t bwd_workspace(int64_t rows, int64_t cols) {  // of any type and alignment
   int64_t z = 1;
   for (int V : {4, 8}) {
-    const Plan p = plan_units(rows, (cols + V - 1) / V, false);
+    const Plan p = plan_units(rows, (cols + V - 1) / V, false, kBwdFill);
     const Plan q = plan_pieces(rows, cols, 16 / V, 2 * kPieceStages + 1);
     for (const int64_t n : {p.ctas, q.ctas, int64_t(p.per && q.per ? 0 : slabs_wide(rows, cols))})
       if (n > z) z = n;
