@@ -123,7 +123,11 @@ template <typename T> __device__ __forceinline__ uint4 no_logits() {  // -inf
 // Distance of a smaller maximum to a larger one, in powers of two; what is there at 2^-1000 is nothing, and the
 // distance stays finite for -inf and for the types' lowest values.
 __device__ __forceinline__ float below(float m, float to, float s) { return fmaxf((m - to) * s, -1000.f); }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(a, fmaxf(b, c)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // out[r] = the key with r larger ones among the n (all different) in `keys`, for r < k.
 __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int n, int k, unsigned long long* out) {
@@ -187,18 +191,18 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
     }
   };
   auto load = [&](int u, uint4 (&q)[kU]) {
+    const uint4* from = units + u + threadIdx.x;
+    if (u + kT * kU <= u1) {
 #pragma unroll
-    for (int j = 0; j < kU; ++j) {
-      const int v = u + j * kT + threadIdx.x;
-      q[j] = v < u1 ? ld_stream(units + v) : no_logits<T>();
+      for (int j = 0; j < kU; ++j) q[j] = ld_stream(from + j * kT);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kU; ++j) q[j] = u + j * kT + int(threadIdx.x) < u1 ? ld_stream(from + j * kT) : no_logits<T>();
     }
   };
-  uint4 q[kU];
-  load(u0, q);
   float group = -CUDART_INF_F;
-  for (int i = 0, u = u0, g = 0; i < rounds; ++i, u += kT * kU) {
-    uint4 next[kU];
-    load(u + kT * kU, next);
+  int g = 0;
+  auto take = [&](uint4 (&q)[kU], int i) {  // round i
     Two f[kU][N];
     float top = -CUDART_INF_F;
 #pragma unroll
@@ -216,7 +220,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
         const Two t = mul2(add2(f[j][n], base), both(s));
         const Two e{exp2_approx(t.a), exp2_approx(t.b)};
         sum = add2(sum, e);
-        if constexpr (kEntropy) dot = fma2(e, Two{fmaxf(t.a, -200.f), fmaxf(t.b, -200.f)}, dot);
+        if constexpr (kEntropy) dot = fma2(e, Two{fmaxf(t.a, -200.f), fmaxf(t.b, -200.f)}, dot);  // t may be -inf, where e is 0
       }
     if constexpr (kTop) {
       group = fmaxf(group, top);
@@ -225,8 +229,15 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
         group = -CUDART_INF_F;
       }
     }
-#pragma unroll
-    for (int j = 0; j < kU; ++j) q[j] = next[j];
+  };
+  uint4 q[kU], next[kU];
+  load(u0, q);
+  for (int i = 0; i < rounds; i += 2) {
+    load(u0 + (i + 1) * kT * kU, next);
+    take(q, i);
+    if (i + 1 == rounds) break;
+    load(u0 + (i + 2) * kT * kU, q);
+    take(next, i + 1);
   }
   if (single >= 0) {
     const float v = to_f32(row.x[single]);
@@ -387,7 +398,7 @@ template <typename T> __device__ __forceinline__ uint4 cut(const uint4& a, const
 }
 
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(kT)
+__global__ void __launch_bounds__(kT, 4)
 logprobs_bwd_kernel(const T* logits, int64_t ld, const int64_t* __restrict__ targets, int64_t ignore, float s,
                     float inv_temp, const float* __restrict__ lse, const float* __restrict__ entropy,
                     const float* __restrict__ g_lp, const float* __restrict__ g_ent, const float* __restrict__ g_lse,
@@ -456,17 +467,30 @@ logprobs_bwd_kernel(const T* logits, int64_t ld, const int64_t* __restrict__ tar
         if (u + j * kT < u1) finish(u + j * kT, q[j]);
     }
   } else {
-    for (int u = u0 + threadIdx.x; u < u1; u += kT) {
-      const T* from = x + out.col(u) - off;  // a multiple of 16
-      uint4 q;
-      if (from >= x && out.col(u) - off + 2 * V <= vocab) {
-        q = cut<T>(__ldg(reinterpret_cast<const uint4*>(from)), __ldg(reinterpret_cast<const uint4*>(from + V)), off);
-      } else {  // a unit that reaches out of the row
-        T* e = reinterpret_cast<T*>(&q);
+    auto whole = [&](int u) { return u < u1 && out.col(u) >= off && out.col(u) - off + 2 * V <= vocab; };
+    for (int u = u0 + threadIdx.x; u < u1; u += kT * kU) {
+      uint4 lo[kU], hi[kU];
 #pragma unroll
-        for (int n = 0; n < V; ++n) e[n] = x[out.col(u) + n];
+      for (int j = 0; j < kU; ++j) {
+        lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
+        if (whole(u + j * kT)) {
+          const T* from = x + out.col(u + j * kT) - off;  // a multiple of 16
+          lo[j] = __ldg(reinterpret_cast<const uint4*>(from));
+          hi[j] = __ldg(reinterpret_cast<const uint4*>(from + V));
+        }
       }
-      finish(u, q);
+#pragma unroll
+      for (int j = 0; j < kU; ++j) {
+        const int v = u + j * kT;
+        if (v >= u1) break;
+        uint4 q = cut<T>(lo[j], hi[j], off);
+        if (!whole(v)) {  // it reaches out of the row
+          T* e = reinterpret_cast<T*>(&q);
+#pragma unroll
+          for (int n = 0; n < V; ++n) e[n] = x[out.col(v) + n];
+        }
+        finish(v, q);
+      }
     }
   }
   if (single >= 0) {
