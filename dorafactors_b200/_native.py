@@ -10,6 +10,7 @@ call fails loudly.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -419,24 +420,20 @@ def weight_norm_dense(W, L, scale: float, norm_out) -> None:
 # Norms, token log probabilities and AdamW.  Their smallest calls are short against
 # the host's own work, so addresses and streams go as plain integers.
 # ---------------------------------------------------------------------------
-def on_device(device: torch.device):
-    """Guard that makes ``device`` current where it is not (a launch goes to the current device)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _call(fn, index: int, *args) -> int:
+    """``fn(*args, stream)`` on device ``index`` (a launch goes to the current device) and its current stream."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-class _SameDevice:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+def _on(index: int):
+    """Guard that makes device ``index`` current where it is not."""
+    return _NOTHING if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
-_SAME_DEVICE = _SameDevice()
-
-
-def _raw_stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+_NOTHING = contextlib.nullcontext()
 
 
 def addr(t: torch.Tensor | None) -> int | None:
@@ -464,59 +461,51 @@ def rows_of(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
 
 
 def layer_norm_fwd(x, rows, cols, ldx, weight, bias, w_code: int, eps: float, y, mean, rstd, rms: bool) -> None:
-    dev = x.device
     lib = load_library()
-    with on_device(dev):
-        if rms:
-            code = lib.dora_rms_norm_fwd(x.data_ptr(), ldx, addr(weight), w_code, eps, y.data_ptr(), addr(rstd), rows,
-                                         cols, DTYPE_CODE[x.dtype], _raw_stream(dev))
-        else:
-            code = lib.dora_layer_norm_fwd(x.data_ptr(), ldx, addr(weight), addr(bias), w_code, eps, y.data_ptr(),
-                                           addr(mean), addr(rstd), rows, cols, DTYPE_CODE[x.dtype], _raw_stream(dev))
+    w = None if weight is None else weight.data_ptr()
+    if rms:
+        code = _call(lib.dora_rms_norm_fwd, x.get_device(), x.data_ptr(), ldx, w, w_code, eps, y.data_ptr(),
+                     rstd.data_ptr(), rows, cols, DTYPE_CODE[x.dtype])
+    else:
+        code = _call(lib.dora_layer_norm_fwd, x.get_device(), x.data_ptr(), ldx, w, addr(bias), w_code, eps,
+                     y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, cols, DTYPE_CODE[x.dtype])
     if code:
         check(code, "dora_rms_norm_fwd" if rms else "dora_layer_norm_fwd")
 
 
 def layer_norm_bwd(dy, lddy, x, ldx, rows, cols, weight, w_code: int, mean, rstd, dx, dw, db, rms: bool) -> None:
-    dev = x.device
+    index = x.get_device()
     lib = load_library()
-    with on_device(dev):
-        ws, nbytes = None, 0
-        if dw is not None or db is not None:
+    ws, nbytes = None, 0
+    if dw is not None or db is not None:
+        with _on(index):
             nbytes = lib.dora_layer_norm_bwd_workspace_size(rows, cols)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        if rms:
-            code = lib.dora_rms_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, addr(weight), w_code, addr(rstd),
-                                         addr(dx), addr(dw), addr(ws), nbytes, rows, cols, DTYPE_CODE[x.dtype],
-                                         _raw_stream(dev))
-        else:
-            code = lib.dora_layer_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, addr(weight), w_code, addr(mean),
-                                           addr(rstd), addr(dx), addr(dw), addr(db), addr(ws), nbytes, rows, cols,
-                                           DTYPE_CODE[x.dtype], _raw_stream(dev))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    if rms:
+        code = _call(lib.dora_rms_norm_bwd, index, dy.data_ptr(), lddy, x.data_ptr(), ldx, addr(weight), w_code,
+                     addr(rstd), addr(dx), addr(dw), addr(ws), nbytes, rows, cols, DTYPE_CODE[x.dtype])
+    else:
+        code = _call(lib.dora_layer_norm_bwd, index, dy.data_ptr(), lddy, x.data_ptr(), ldx, addr(weight), w_code,
+                     addr(mean), addr(rstd), addr(dx), addr(dw), addr(db), addr(ws), nbytes, rows, cols,
+                     DTYPE_CODE[x.dtype])
     if code:
         check(code, "dora_rms_norm_bwd" if rms else "dora_layer_norm_bwd")
 
 
 def token_logprobs_fwd(logits, ld, targets, ignore_index: int, temperature: float, logprobs, lse, entropy, top_k: int,
                        top_logprobs, top_indices, rows: int, vocab: int) -> None:
-    dev = logits.device
-    with on_device(dev):
-        code = load_library().dora_token_logprobs_fwd(
-            logits.data_ptr(), ld, targets.data_ptr(), ignore_index, temperature, logprobs.data_ptr(), lse.data_ptr(),
-            addr(entropy), top_k, addr(top_logprobs), addr(top_indices), rows, vocab, DTYPE_CODE[logits.dtype],
-            _raw_stream(dev))
+    code = _call(load_library().dora_token_logprobs_fwd, logits.get_device(), logits.data_ptr(), ld,
+                 targets.data_ptr(), ignore_index, temperature, logprobs.data_ptr(), lse.data_ptr(), addr(entropy),
+                 top_k, addr(top_logprobs), addr(top_indices), rows, vocab, DTYPE_CODE[logits.dtype])
     if code:
         check(code, "dora_token_logprobs_fwd")
 
 
 def token_logprobs_bwd(logits, ld, targets, ignore_index: int, temperature: float, lse, entropy, g_logprobs,
                        g_entropy, g_lse, d_logits, ld_d: int, rows: int, vocab: int) -> None:
-    dev = logits.device
-    with on_device(dev):
-        code = load_library().dora_token_logprobs_bwd(
-            logits.data_ptr(), ld, targets.data_ptr(), ignore_index, temperature, lse.data_ptr(), addr(entropy),
-            addr(g_logprobs), addr(g_entropy), addr(g_lse), d_logits.data_ptr(), ld_d, rows, vocab,
-            DTYPE_CODE[logits.dtype], _raw_stream(dev))
+    code = _call(load_library().dora_token_logprobs_bwd, logits.get_device(), logits.data_ptr(), ld,
+                 targets.data_ptr(), ignore_index, temperature, lse.data_ptr(), addr(entropy), addr(g_logprobs),
+                 addr(g_entropy), addr(g_lse), d_logits.data_ptr(), ld_d, rows, vocab, DTYPE_CODE[logits.dtype])
     if code:
         check(code, "dora_token_logprobs_bwd")
 
@@ -529,18 +518,14 @@ ADAMW_TENSOR = [("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg_sq
 def adamw_step(table: int, count: int, dtype: torch.dtype, state_bits: int, lr: float, betas, eps: float,
                weight_decay: float, step: int, device: torch.device) -> None:
     """``table``: the host address of ``count`` contiguous ``ADAMW_TENSOR`` records."""
-    with on_device(device):
-        code = load_library().dora_adamw_step(table, count, DTYPE_CODE[dtype], state_bits, lr,
-                                              betas[0], betas[1], eps, weight_decay, step, _raw_stream(device))
+    code = _call(load_library().dora_adamw_step, device.index, table, count, DTYPE_CODE[dtype], state_bits, lr,
+                 betas[0], betas[1], eps, weight_decay, step)
     if code:
         check(code, "dora_adamw_step")
 
 
 def adamw_decode(m_codes, m_scale, v_codes, v_scale, m, v) -> None:
-    dev = m.device
-    with on_device(dev):
-        code = load_library().dora_adamw_decode(m_codes.data_ptr(), m_scale.data_ptr(), v_codes.data_ptr(),
-                                                v_scale.data_ptr(), m.data_ptr(), v.data_ptr(), m.numel(),
-                                                _raw_stream(dev))
+    code = _call(load_library().dora_adamw_decode, m.get_device(), m_codes.data_ptr(), m_scale.data_ptr(),
+                 v_codes.data_ptr(), v_scale.data_ptr(), m.data_ptr(), v.data_ptr(), m.numel())
     if code:
         check(code, "dora_adamw_decode")

@@ -55,11 +55,10 @@ def _forward(x, weight, bias, eps, rms: bool, what: str):
         raise ValueError(f"{what}: eps must not be negative, got {eps}")
     w, b, code = _params(x, shape[-1], weight, bias, what)
     data, rows, cols, ld = _native.rows_of(x)
-    device = x.device
-    y = torch.empty(shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x) if data is x and ld == cols else x.new_empty(shape)
     lead = shape[:-1]
-    rstd = torch.empty(lead, dtype=torch.float32, device=device)
-    mean = None if rms else torch.empty(lead, dtype=torch.float32, device=device)
+    rstd = x.new_empty(lead, dtype=torch.float32)
+    mean = None if rms else x.new_empty(lead, dtype=torch.float32)
     if rows and cols:
         _native.layer_norm_fwd(data, rows, cols, ld, w, b, code, eps, y, mean, rstd, rms)
     return y, mean, rstd
