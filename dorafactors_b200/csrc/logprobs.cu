@@ -382,21 +382,6 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
 // Backward: one pass, a CTA to a part of a row; bound by HBM.  The units are those of the
 // output; where the logits' rows stand differently to 16 bytes, each is cut out of two of theirs.
 // ---------------------------------------------------------------------------
-// V elements from column c on: c's 16-byte unit and the one after it, shifted by `off` elements.
-template <typename T> __device__ __forceinline__ uint4 cut(const uint4& a, const uint4& b, int off) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  uint32_t o[5];
-  switch (sizeof(T) == 4 ? off : off / 2) {  // the same for the whole row
-    case 0: for (int i = 0; i < 5; ++i) o[i] = w[i]; break;
-    case 1: for (int i = 0; i < 5; ++i) o[i] = w[i + 1]; break;
-    case 2: for (int i = 0; i < 5; ++i) o[i] = w[i + 2]; break;
-    default: for (int i = 0; i < 5; ++i) o[i] = w[i + 3]; break;
-  }
-  if (sizeof(T) == 2 && (off & 1))
-    for (int i = 0; i < 4; ++i) o[i] = __byte_perm(o[i], o[i + 1], 0x5432);
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
 template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kT, 4)
 logprobs_bwd_kernel(const T* logits, int64_t ld, const int64_t* __restrict__ targets, int64_t ignore, float s,

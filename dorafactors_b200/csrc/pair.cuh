@@ -78,6 +78,22 @@ template <typename T> struct Pairs {
   }
 };
 
+// The 16 bytes that start `off` elements of T (0 .. a vector less one; the same for all threads) after a's first, of a and
+// the vector b after it.
+template <typename T> __device__ __forceinline__ uint4 cut(const uint4& a, const uint4& b, int off) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t o[5];
+  switch (sizeof(T) == 4 ? off : off / 2) {
+    case 0: for (int i = 0; i < 5; ++i) o[i] = w[i]; break;
+    case 1: for (int i = 0; i < 5; ++i) o[i] = w[i + 1]; break;
+    case 2: for (int i = 0; i < 5; ++i) o[i] = w[i + 2]; break;
+    default: for (int i = 0; i < 5; ++i) o[i] = w[i + 3]; break;
+  }
+  if (sizeof(T) == 2 && (off & 1))
+    for (int i = 0; i < 4; ++i) o[i] = __byte_perm(o[i], o[i + 1], 0x5432);
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 // A 16-byte copy to shared memory that runs on its own; a thread that reads back only what it has copied
 // itself needs no barrier, just copies_done.
 __device__ __forceinline__ void copy_async16(uint32_t to, const void* from) {
