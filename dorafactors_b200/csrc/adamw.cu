@@ -16,6 +16,9 @@
 //      hashed bits: with b2 = 0.999 a step changes v by less than half a code, which
 //      rounding to nearest would lose every time.  A v > 0 never becomes 0, since
 //      sqrt(v) = 0 would leave only eps in the denominator.
+//
+// Measured over 672 tensors, 337M elements: fp32 1459 us (HBM, 0.99 of the copy rate); bf16 with 8-bit moments
+// 783 us (the ALU pipe, 75 % busy; HBM alone would take 517 us), their values 508 us (HBM).
 #include <cfloat>
 #include <type_traits>
 
