@@ -260,7 +260,7 @@ ln_fwd_kernel(const TA* __restrict__ x, int64_t ldx, const void* __restrict__ w,
 
 // Backward: one pass over dy and x, with the columns' sums for d_weight and d_bias in
 // registers; they cost no traffic but one partial row a CTA.  bf16: RMS norm at 32768 x 4096
-// 127 us (HBM, 0.97 of the copy rate), layer norm at 16384 x 8192 168 us (0.73: issue slots, with
+// 135 us (HBM, 0.91 of the copy rate), layer norm at 16384 x 8192 176 us (0.70: issue slots, with
 // the 16 warps an SM that 128 registers leave).
 template <typename TA, bool kRms, int PER, int S, int kMax, bool kCols>
 __global__ void __launch_bounds__(kMax)

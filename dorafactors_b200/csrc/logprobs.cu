@@ -382,7 +382,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __r
 }
 
 // ---------------------------------------------------------------------------
-// Backward: one pass, a CTA to a part of a row; bound by HBM (4096 x 128256 bf16, a tenth ignored: 324 us, 0.94
+// Backward: one pass, a CTA to a part of a row; bound by HBM (4096 x 128256 bf16, a tenth ignored: 331 us, 0.92
 // of the copy rate).  The units are those of the
 // output; where the logits' rows stand differently to 16 bytes, each is cut out of two of theirs.
 // ---------------------------------------------------------------------------
